@@ -188,15 +188,9 @@ KH_EXPORT int hipK_init(int device_id) {
              chosen, prop.gcnArchName);
     return KH_ERR_INVALID_ARG;
   }
-  {
-    // the library's default stream carries the chain of dependent kernels: give it the highest
-    // priority, so that its (short) kernels are not queued behind work of the other streams
-    int lo = 0, hi = 0;
-    KH_HIP(hipDeviceGetStreamPriorityRange(&lo, &hi));
-    const char *e = getenv("KALDI_HIP_STREAM_PRIO");
-    if (e && atoi(e) == 0) KH_HIP(hipStreamCreateWithFlags(&c.stream, hipStreamNonBlocking));
-    else KH_HIP(hipStreamCreateWithPriority(&c.stream, hipStreamNonBlocking, hi));
-  }
+  // One priority for every stream: work on streams of different priorities has been seen to hang, and the training
+  // steps measure the same without.
+  KH_HIP(hipStreamCreateWithFlags(&c.stream, hipStreamNonBlocking));
   {
     int st = kh::static_scratch_setup(chosen);
     if (st != KH_OK) return st;
@@ -249,11 +243,7 @@ KH_EXPORT int hipK_stream_create(khStream_t *stream) {
   KH_CHECK_INIT();
   KH_REQUIRE(stream != nullptr);
   hipStream_t s;
-  int lo = 0, hi = 0;
-  KH_HIP(hipDeviceGetStreamPriorityRange(&lo, &hi));
-  const char *e = getenv("KALDI_HIP_STREAM_PRIO");
-  if (e && atoi(e) == 0) KH_HIP(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
-  else KH_HIP(hipStreamCreateWithPriority(&s, hipStreamNonBlocking, lo));  // lowest: see hipK_init
+  KH_HIP(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
   *stream = (khStream_t)s;
   return KH_OK;
 }
