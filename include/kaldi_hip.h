@@ -460,6 +460,96 @@ int hipF_affine_forward_xent(khStream_t s, int trans_w, int32_t N, int32_t O, in
 int hipF_mse_eval(khStream_t s, const float *a, const float *b, float *diff, float *row_sq, double *loss,
                   MatrixDim d);
 
+/* ------------------------------------------------------------------------------------------
+ * Low-rank adapters of many speakers beside one shared affine layer (no counterpart in the reference).
+ * Adapter g adds  s_g * (in * down_g^T) * up_g  to the rows that belong to it.  The adapters of a layer lie
+ * below each other in two matrices: rows begin[g] .. begin[g+1]-1 of `down` (x I) and of `up` (x O) are
+ * adapter g, so they may have different ranks (0 included) and a CuMatrix holds either stack.  Both stacks
+ * together are stepped by hipF_add_mat / hipF_sgd_apply_flat like any other weights.
+ * begin[] lives on the device and is not checked by the host: the kernels never leave rows 0 .. rows-1 of the
+ * stacks, and an adapter whose range is longer than max_rank is cut there.
+ * ------------------------------------------------------------------------------------------ */
+#define KH_MAX_ADAPTER_RANK 128
+typedef struct {
+  int32_t num;          /* adapters; 0 = none (the layer alone) */
+  int32_t max_rank;     /* no adapter has more rows: 1 .. KH_MAX_ADAPTER_RANK */
+  int32_t rows;         /* rows of down and of up */
+  const int32_t *begin; /* device, num + 1, ascending */
+  const float *scale;   /* device, num; NULL = 1 */
+  const float *down; int32_t lddown; /* rows x I */
+  const float *up; int32_t ldup;     /* rows x O */
+} khAdapters;
+
+/* Groups the N rows of a bunch by adapter: order[] lists the rows of adapter 0, then of adapter 1, ..., each in
+ * ascending order, then the rows without one (row_adapter[r] outside [0, num)); adapter g's are
+ * order[row_begin[g] .. row_begin[g+1]-1].  order: N, row_begin: num + 1 int32 on the device.  One bunch's grouping
+ * serves every layer, forward and backward. */
+int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int32_t num, int32_t *order,
+                        int32_t *row_begin);
+
+/* hipF_affine_forward(act, KH_TRANS, ...) with adapters:
+ *   t(N x max_rank)  t[r,k]   = s_g * sum_i in[r,i] * down[begin[g]+k, i]      (0 for k >= the adapter's rank, and
+ *                                                                               for a row without an adapter)
+ *   out(N x O)       out[r,:] = act( bias + in[r,:] * W^T + t[r,:] * up_g )
+ * with g = row_adapter[r].  `order` (may be NULL: the rows as they stand) is the sequence in which rows are put
+ * together into tiles: give hipI32_adapter_plan's where neighbouring rows have different adapters, NULL where they lie
+ * together already (utterances, single frames).  The result does not depend on it beyond rounding.  `t` is what
+ * the backward pass needs; bias may be NULL.  out and t must not overlap an input.  Rows behind N and columns
+ * behind O (max_rank) are left as they are.  Uses no library workspace: may be captured into a graph.
+ * Arithmetic: every float is taken as the sum of three bfloat16 numbers (24 bits of mantissa: exact) and a product
+ * of two floats as the six largest of the nine part products, on the matrix cores with float sums; what is left out
+ * is below 2^-26 of the product, less than one rounding of a float product.  An infinity or NaN in a row of `in`
+ * makes that row of t and out NaN (of `act` NaN); it does not reach other rows. */
+int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, int32_t I, const float *in, int32_t ldin,
+                         const float *W, int32_t ldw, const float *bias, const khAdapters *ad,
+                         const int32_t *row_adapter, const int32_t *order, float *t, int32_t ldt, float *out,
+                         int32_t ldout);
+
+/* The backward pass, e(N x O) = error at the affine layer's output (before the activation):
+ *   u(N x max_rank)    u[r,k]    = s_g * sum_o e[r,o] * up[begin[g]+k, o]       (0 where t is 0)
+ *   eout(N x I)        eout[r,:] = ( e[r,:] * W + u[r,:] * down_g ) [ .* y .* (1-y) when y != NULL ]
+ *   gdown(rows x I)    gdown[begin[g]+k, :] = sum over the rows r of g of  u[r,k] * in[r,:]
+ *   gup(rows x O)      gup  [begin[g]+k, :] = sum over the rows r of g of  t[r,k] * e[r,:]
+ * eout may be NULL (the lowest layer), gdown and gup may be NULL (frozen adapters; then `in`, `t` may be NULL too).
+ * order / row_begin: hipI32_adapter_plan of the same rows; order must be a permutation of 0 .. N-1 for the
+ * gradients to be whole (an entry outside is skipped).  An adapter without rows gets a gradient of zeros; rows of the
+ * stacks outside every adapter are left as they are.  Sums are taken in a fixed order: the same call gives the same
+ * bits.  Outputs must not overlap an input.  The shared W is not updated here (hipF_affine_update). */
+int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t I, const float *e, int32_t lde, const float *in,
+                          int32_t ldin, const float *W, int32_t ldw, const khAdapters *ad, const int32_t *row_adapter,
+                          const int32_t *order, const int32_t *row_begin, const float *t, int32_t ldt, float *u,
+                          int32_t ldu, const float *y, int32_t ldy, float *eout, int32_t ldeout, float *gdown,
+                          int32_t ldgdown, float *gup, int32_t ldgup);
+
+/* ------------------------------------------------------------------------------------------
+ * Learning from another network's outputs (no counterpart in the reference, whose trainers know hard labels and
+ * target matrices).
+ * ------------------------------------------------------------------------------------------ */
+#define KH_MAX_TOP 128
+/* The K largest elements of every row (1 <= K <= KH_MAX_TOP) in descending order, equal ones by ascending column,
+ * NaN above every number: idx[r,k] = column, val[r,k] = mat[r, idx[r,k]].  K beyond the row's length fills up with
+ * idx -1, val -inf.  lse[r] = log(sum_c exp(mat[r,c])) (may be NULL; -inf for a row of -inf, NaN for
+ * one that holds a NaN or +inf), so that val - lse are log-posteriors.  What hipF_find_row_max_id is for one
+ * maximum; it makes a teacher's outputs small enough to keep.  Uses no library workspace. */
+int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t K, int32_t *idx, int32_t ldidx, float *val,
+                 int32_t ldval, float *lse);
+
+/* Loss and gradient of a network's output towards a teacher's K largest logits, mixed with hard labels; x(rows x cols)
+ * are the network's outputs BEFORE the softmax.  Per row, with T = temperature and h = hard_weight:
+ *   q = softmax of val / T over the row's entries with 0 <= idx < cols   (others are not there; none: q = 0)
+ *   p = softmax(x / T), p1 = softmax(x)
+ *   row_loss = w * [ (1-h) * T^2 * sum_k q_k (log q_k - log p[idx_k])  +  h * (-log p1[label]) ]
+ *   diff     = w * [ (1-h) * T * (p * (1 if there is an entry else 0) - q)  +  h * (p1 - onehot(label)) ]
+ * diff is the derivative of row_loss with respect to x; it may be NULL (the loss alone) or alias x.  A column named by two
+ * entries gets both; an entry of -inf has q = 0 and 0 * log 0 = 0.  label (may be NULL when h is 0): a label outside
+ * [0, cols) is none, its part of the row is zero.  w = weight[r] (NULL = 1); a row of weight 0, and a row whose x are
+ * all -inf, get loss 0 and a gradient of zeros whatever the row holds.  row_loss (rows floats) may be NULL if loss is;
+ * loss[0] += sum of row_loss (double on the device, summed in row order; may be NULL).  T > 0, 0 <= h <= 1.
+ * Sums in float over at most 1024 partial sums per row, the logarithms in double.  Uses no library workspace. */
+int hipF_distill_eval(khStream_t s, const float *x, MatrixDim d, const int32_t *idx, int32_t ldidx, const float *val,
+                      int32_t ldval, int32_t K, const int32_t *label, const float *weight, float temperature,
+                      float hard_weight, float *diff, int32_t lddiff, float *row_loss, double *loss);
+
 /* Rbm::RbmUpdate (nnet-rbm.h:178-223):
  *   dW = mom*dW - (lr/N) neg_hid^T neg_vis + (lr/N) pos_hid^T pos_vis - lr*l2*W ;  W += dW
  *   da = mom*da - (lr/N) colsum(neg_vis) + (lr/N) colsum(pos_vis) ;              a += da

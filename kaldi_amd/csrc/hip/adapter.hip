@@ -1,0 +1,604 @@
+// Low-rank adapters of many speakers beside one shared affine layer: hipI32_adapter_plan, hipF_adapter_forward,
+// hipF_adapter_backward (include/kaldi_hip.h has the formulas).
+//
+// A float product on this chip's fp32 matrix instructions is bound at 157 TFLOP/s; on bfloat16 they do 2.5 PFLOP/s.
+// So every operand is split, where it is loaded, into three bfloat16 numbers that add up to it exactly (8 bits of
+// mantissa each, rounded to nearest: |x - hi| <= 2^-9 |x|, |x - hi - mid| <= 2^-18 |x|, the rest fits lo), and a product
+// is the sum of the six part products down to 2^-18 of it, accumulated in float by the matrix instruction: the bfloat16x3
+// decomposition published by Henry, Tang and Heinecke (2019).  The three products left out are at most
+// 2 * 2^-27 + 2^-36 of the product, an eighth of a float's rounding.  An infinity splits into inf + NaN.
+#include <algorithm>
+
+#include "common.h"
+
+namespace {
+
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+
+// ---- eight floats as three fragments of eight bfloat16 ----------------------------------------------------------
+struct Frag {
+  v8b hi, mid, lo;
+};
+__device__ __forceinline__ Frag split8(const float (&x)[8]) {
+  Frag f;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const v2f v = {x[i], x[i + 1]};
+    const v2b h = __builtin_convertvector(v, v2b);
+    const v2f r = {v.x - (float)h.x, v.y - (float)h.y};
+    const v2b m = __builtin_convertvector(r, v2b);
+    const v2f q = {r.x - (float)m.x, r.y - (float)m.y};
+    const v2b l = __builtin_convertvector(q, v2b);
+    f.hi[i] = h.x, f.hi[i + 1] = h.y;
+    f.mid[i] = m.x, f.mid[i + 1] = m.y;
+    f.lo[i] = l.x, f.lo[i + 1] = l.y;
+  }
+  return f;
+}
+// c += a * b, smallest part products first
+__device__ __forceinline__ v4f mfma6(const Frag &a, const Frag &b, v4f c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, b.hi, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.lo, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.mid, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.hi, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.mid, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.hi, c, 0, 0, 0);
+  return c;
+}
+
+// ---- operand loads ------------------------------------------------------------------------------------------------
+// The 16x16x32 instruction: lane l holds A[l % 16][8 (l / 16) + e] and B[8 (l / 16) + e][l % 16], e = 0..7, and gets
+// D[4 (l / 16) + i][l % 16], i = 0..3.
+
+// eight floats of one row, k .. k+7, zeros from K on
+template <bool VEC>
+__device__ __forceinline__ void load_row8(const float *row, int k, int K, float (&x)[8]) {
+  if (VEC && k + 8 <= K) {
+    const v4f a = *reinterpret_cast<const v4f *>(row + k), b = *reinterpret_cast<const v4f *>(row + k + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = k + e < K ? row[k + e] : 0.f;
+  }
+}
+// NB neighbouring floats of a row from column c, zeros from C on
+template <int NB, bool VEC>
+__device__ __forceinline__ void load_cols(const float *row, int c, int C, float (&x)[NB]) {
+  if (VEC && NB == 4 && c + 4 <= C) {
+    const v4f a = *reinterpret_cast<const v4f *>(row + c);
+    x[0] = a.x, x[1 % NB] = a.y, x[2 % NB] = a.z, x[3 % NB] = a.w;
+  } else if (VEC && NB == 2 && c + 2 <= C) {
+    const v2f a = *reinterpret_cast<const v2f *>(row + c);
+    x[0] = a.x, x[1 % NB] = a.y;
+  } else {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) x[j] = c + j < C ? row[c + j] : 0.f;
+  }
+}
+
+// ---- which adapter ------------------------------------------------------------------------------------------------
+struct Stack {
+  int num, max_rank, rows;
+  const int32_t *begin;
+  const float *scale;
+};
+// the stack rows of adapter g (0 <= g < num): first row and how many, inside the stack whatever begin[] holds
+__device__ __forceinline__ void stack_rows(const Stack &st, int g, int *first, int *rank) {
+  int lo = st.begin[g], hi = st.begin[g + 1];
+  lo = min(max(lo, 0), st.rows);
+  hi = min(hi, st.rows);
+  *first = lo;
+  *rank = max(0, min(hi - lo, st.max_rank));
+}
+
+// Row `i` of the tile sequence: the row itself or order[i]; -1 behind the end or outside the matrix.
+__device__ __forceinline__ int row_of(const int32_t *order, int i, int N) {
+  if (i >= N) return -1;
+  if (!order) return i;
+  const int r = order[i];
+  return (unsigned)r < (unsigned)N ? r : -1;
+}
+__device__ __forceinline__ int adapter_of(const int32_t *row_adapter, int num, int row) {
+  if (row < 0 || num == 0) return -1;
+  const int g = row_adapter[row];
+  return (unsigned)g < (unsigned)num ? g : -1;
+}
+
+// The runs of equal adapters among the (up to 64) rows of a tile, as every lane of a wave sees them: lane m has the
+// adapter of tile row m.  `starts` marks the first rows of runs that have an adapter, `changes` the first rows of all.
+struct Runs {
+  unsigned long long starts, changes;
+};
+__device__ __forceinline__ Runs find_runs(int g, int lane) {
+  const int prev = __shfl_up(g, 1, 64);
+  const bool change = lane == 0 || prev != g;
+  Runs r;
+  r.changes = __ballot(change);
+  r.starts = __ballot(change && g >= 0);
+  return r;
+}
+// rows of the run that starts at bit s
+__device__ __forceinline__ unsigned long long run_mask(const Runs &r, int s) {
+  const unsigned long long above = s == 63 ? 0ull : (r.changes >> (s + 1)) << (s + 1);
+  const unsigned long long from = ~0ull << s;
+  return above ? from & ((above & (0ull - above)) - 1ull) : from;
+}
+
+// ---- grouping of a bunch --------------------------------------------------------------------------------------------
+// One workgroup per adapter (and one for the rows without): counts the rows in front of its group, then writes its rows
+// in ascending order.  Every workgroup reads all ids (from the L2: N * (num + 1) * 8 bytes in all); no atomics, no
+// scratch, a stable order.
+__global__ __launch_bounds__(1024) void plan_kernel(const int32_t *row_adapter, int N, int num, int32_t *order,
+                                                    int32_t *row_begin) {
+  __shared__ int part[16];
+  const int me = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  int before = 0;
+  for (int i = threadIdx.x; i < N; i += blockDim.x) {
+    const unsigned g = (unsigned)row_adapter[i];
+    before += (g < (unsigned)num ? (int)g : num) < me;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+  if (lane == 0) part[wave] = before;
+  __syncthreads();
+  int at = 0;
+  for (int w = 0; w < waves; ++w) at += part[w];
+  __syncthreads();
+  if (threadIdx.x == 0) row_begin[me] = at;
+  for (int i0 = 0; i0 < N; i0 += blockDim.x) {
+    const int i = i0 + threadIdx.x;
+    bool mine = false;
+    if (i < N) {
+      const unsigned g = (unsigned)row_adapter[i];
+      mine = (g < (unsigned)num ? (int)g : num) == me;
+    }
+    const unsigned long long hits = __ballot(mine);
+    if (lane == 0) part[wave] = __popcll(hits);
+    __syncthreads();
+    int place = at;
+    for (int w = 0; w < waves; ++w) {
+      if (w < wave) place += part[w];
+      at += part[w];
+    }
+    if (mine) order[place + __popcll(hits & ((1ull << lane) - 1ull))] = i;
+    __syncthreads();
+  }
+}
+
+// ---- the narrow product: t = s_g * x * side_g^T ----------------------------------------------------------------------
+// One workgroup per window of up to 16 rows and block of 16 * NB rank columns; its NW waves take steps of 32 of the
+// inner dimension in turn and add up through LDS in a fixed order.  A window of several adapters is gone through
+// once per run of equal adapters; only the run's rows are kept from a pass, so nothing of one row reaches another.
+template <int NB, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW) void narrow_kernel(const float *x, int ldx, int N, int K, const float *side, int lds,
+                                                         Stack st, const int32_t *row_adapter, const int32_t *order,
+                                                         int window, float *t, int ldt) {
+  __shared__ float part[NW][16][16 * NB + 4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, q = lane >> 4;
+  const int first_row = blockIdx.x * window, col0 = blockIdx.y * 16 * NB;
+  const int row = lane < window ? row_of(order, first_row + lane, N) : -1;
+  const int g = adapter_of(row_adapter, st.num, row);
+  const Runs runs = find_runs(g, lane);
+  const int my_row = __shfl(row, l15, 64);
+  const float *xr = x + (size_t)max(my_row, 0) * ldx;
+  v4f total[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) total[j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  for (unsigned long long left = runs.starts; left; left &= left - 1ull) {
+    const int s = __builtin_ctzll(left);
+    const unsigned long long mask = run_mask(runs, s);
+    int lo, rank;
+    stack_rows(st, __shfl(g, s, 64), &lo, &rank);
+    if (rank <= col0) continue;
+    const float *br[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) br[j] = side + (size_t)(lo + min(col0 + NB * l15 + j, rank - 1)) * lds;
+    v4f acc[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 32 * wave; k0 < K; k0 += 32 * NW) {
+      float a[8], b[NB][8];
+      load_row8<VEC>(xr, k0 + 8 * q, K, a);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) load_row8<VEC>(br[j], k0 + 8 * q, K, b[j]);
+      const Frag fa = split8(a);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[j] = mfma6(fa, split8(b[j]), acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if ((mask >> (4 * q + i)) & 1ull && col0 + NB * l15 + j < rank) total[j][i] = acc[j][i];
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][4 * q + i][NB * l15 + j] = total[j][i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < window * 16 * NB; e += 64 * NW) {
+    const int m = e / (16 * NB), c = e % (16 * NB);
+    const int r = row_of(order, first_row + m, N);
+    if (r < 0 || col0 + c >= st.max_rank) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += part[w][m][c];
+    const int ga = adapter_of(row_adapter, st.num, r);
+    if (ga >= 0 && st.scale) v *= st.scale[ga];
+    t[(size_t)r * ldt + col0 + c] = v;
+  }
+}
+
+// ---- the wide product with the adapters' part -----------------------------------------------------------------------
+struct WideArgs {
+  const float *x; int ldx;       // rows x K
+  const float *w; int ldw;       // NN: K x C, else C x K
+  int N, K, C;
+  const float *bias;             // C or null
+  const float *t; int ldt;       // rows x max_rank (null: no adapters)
+  const float *side; int ldside; // stack x C
+  Stack st;
+  const int32_t *row_adapter, *order;
+  const float *y; int ldy;       // derivative of the sigmoid below, or null
+  int act;
+  float *out; int ldout;
+  int tiles_m, tiles_n;
+};
+
+// One workgroup per tile of 16 * MB rows and 16 * NB columns; its NW waves take steps of 32 of the inner dimension in
+// turn, each straight from memory into the registers of the matrix instruction (no wave needs what another loads),
+// and add up through LDS in a fixed order.  The columns of a lane are neighbours: block j of the tile holds columns
+// NB * l + j.  The adapters' part follows in the same way, the runs of equal adapters taken in turn by the waves: a run's
+// product with its rows of the stack is added to the run's rows only.
+template <int MB, int NB, int NW, bool NN, bool VEC>
+__global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
+  constexpr int BM = 16 * MB, BN = 16 * NB;
+  __shared__ float part[NW][BM][BN];
+  // tiles of the same columns run on one of the 8 dies, so that a piece of W comes into one L2 only
+  const int die = blockIdx.x & 7, local = blockIdx.x >> 3;
+  const int tile_n = die + 8 * (local / p.tiles_m), tile_m = local % p.tiles_m;
+  if (tile_n >= p.tiles_n) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, q = lane >> 4;
+  const int m0 = tile_m * BM, n0 = tile_n * BN, c0 = n0 + NB * l15;
+  const int row = lane < BM ? row_of(p.order, m0 + lane, p.N) : -1;
+  int my_row[MB];
+  const float *xr[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    my_row[b] = __shfl(row, 16 * b + l15, 64);
+    xr[b] = p.x + (size_t)max(my_row[b], 0) * p.ldx;
+  }
+  v4f acc[MB][NB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[b][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+
+  const float *wr[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) wr[j] = p.w + (size_t)min(c0 + j, p.C - 1) * p.ldw;
+  for (int k0 = 32 * wave; k0 < p.K; k0 += 32 * NW) {
+    float a[MB][8], b[NB][8];
+#pragma unroll
+    for (int m = 0; m < MB; ++m) load_row8<VEC>(xr[m], k0 + 8 * q, p.K, a[m]);
+    if (NN) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int k = k0 + 8 * q + e;
+        float v[NB] = {};
+        if (k < p.K) load_cols<NB, VEC>(p.w + (size_t)k * p.ldw, c0, p.C, v);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) b[j][e] = v[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) load_row8<VEC>(wr[j], k0 + 8 * q, p.K, b[j]);
+    }
+    Frag fa[MB];
+#pragma unroll
+    for (int m = 0; m < MB; ++m) fa[m] = split8(a[m]);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const Frag fb = split8(b[j]);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) acc[m][j] = mfma6(fa[m], fb, acc[m][j]);
+    }
+  }
+
+  if (p.t) {
+    const int g = adapter_of(p.row_adapter, p.st.num, row);
+    const Runs runs = find_runs(g, lane);
+    int turn = 0;
+    for (unsigned long long left = runs.starts; left; left &= left - 1ull, ++turn) {
+      if (turn % NW != wave) continue;
+      const int s = __builtin_ctzll(left);
+      const unsigned long long mask = run_mask(runs, s);
+      int lo, rank;
+      stack_rows(p.st, __shfl(g, s, 64), &lo, &rank);
+      v4f d[MB][NB];
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) d[m][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+      for (int k0 = 0; k0 < rank; k0 += 32) {
+        float b[NB][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int k = k0 + 8 * q + e;
+          float v[NB] = {};
+          if (k < rank) load_cols<NB, VEC>(p.side + (size_t)(lo + k) * p.ldside, c0, p.C, v);
+#pragma unroll
+          for (int j = 0; j < NB; ++j) b[j][e] = v[j];
+        }
+        Frag fa[MB];
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+          float a[8];
+          load_row8<VEC>(p.t + (size_t)max(my_row[m], 0) * p.ldt, k0 + 8 * q, rank, a);
+          fa[m] = split8(a);
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const Frag fb = split8(b[j]);
+#pragma unroll
+          for (int m = 0; m < MB; ++m) d[m][j] = mfma6(fa[m], fb, d[m][j]);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((mask >> (16 * m + 4 * q + i)) & 1ull) acc[m][j][i] += d[m][j][i];
+    }
+  }
+
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) part[wave][16 * m + 4 * q + i][NB * l15 + j] = acc[m][j][i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < BM * BN; e += 64 * NW) {
+    const int m = e / BN, c = n0 + e % BN;
+    const int r = row_of(p.order, m0 + m, p.N);
+    if (r < 0 || c >= p.C) continue;
+    float v = p.bias ? p.bias[c] : 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) sum += part[w][m][e % BN];
+    v += sum;
+    if (p.act == KH_ACT_SIGMOID) v = kh::sigmoidf(v);
+    if (p.y) {
+      const float yv = p.y[(size_t)r * p.ldy + c];
+      v = v * yv * (1.f - yv);
+    }
+    p.out[(size_t)r * p.ldout + c] = v;
+  }
+}
+
+// ---- gradients of the stacks ----------------------------------------------------------------------------------------
+// g_side[begin + k, c] = sum over the rows r of an adapter of narrow[r, k] * wide[r, c].  One workgroup per adapter,
+// block of 16 * NB columns and block of 16 rank rows; its waves take steps of 32 rows in turn.
+struct GradArgs {
+  const float *narrow; int ldnarrow;
+  const float *wide; int ldwide; int C;
+  float *grad; int ldgrad;
+};
+template <int NB, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW) void grad_kernel(GradArgs down, GradArgs up, int N, Stack st, const int32_t *order,
+                                                       const int32_t *row_begin, int col_tiles, int rank_blocks) {
+  __shared__ float part[NW][16][16 * NB];
+  const bool is_up = blockIdx.y >= (unsigned)rank_blocks;
+  const GradArgs &p = is_up ? up : down;
+  const int k_base = (blockIdx.y - (is_up ? rank_blocks : 0)) * 16;
+  const int g = blockIdx.x / col_tiles, n0 = (blockIdx.x % col_tiles) * 16 * NB;
+  if (n0 >= p.C) return;
+  int lo, rank;
+  stack_rows(st, g, &lo, &rank);
+  if (k_base >= rank) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, q = lane >> 4;
+  const int begin = min(max(row_begin[g], 0), N), end = min(row_begin[g + 1], N), c0 = n0 + NB * l15;
+  v4f acc[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) acc[j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  for (int r0 = begin + 32 * wave; r0 < end; r0 += 32 * NW) {
+    const int mine = lane < 32 && r0 + lane < end ? row_of(order, r0 + lane, N) : -1;
+    float a[8], b[NB][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int r = __shfl(mine, 8 * q + e, 64);
+      a[e] = r >= 0 && k_base + l15 < rank ? p.narrow[(size_t)r * p.ldnarrow + k_base + l15] : 0.f;
+      float v[NB] = {};
+      if (r >= 0) load_cols<NB, VEC>(p.wide + (size_t)r * p.ldwide, c0, p.C, v);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) b[j][e] = v[j];
+    }
+    const Frag fa = split8(a);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[j] = mfma6(fa, split8(b[j]), acc[j]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) part[wave][4 * q + i][NB * l15 + j] = acc[j][i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < 256 * NB; e += 64 * NW) {
+    const int k = e / (16 * NB), c = e % (16 * NB);
+    if (k_base + k >= rank || n0 + c >= p.C) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += part[w][k][c];
+    p.grad[(size_t)(lo + k_base + k) * p.ldgrad + n0 + c] = v;
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------
+bool vec_ok(const float *p, int ld) { return p == nullptr || (kh::aligned16(p) && ld % 4 == 0); }
+
+Stack stack_of(const khAdapters &ad) {
+  Stack st = {ad.num, ad.max_rank, ad.rows, ad.begin, ad.scale};
+  return st;
+}
+
+template <bool VEC>
+void launch_narrow(hipStream_t st, const float *x, int ldx, int N, int K, const float *side, int ldside, const Stack &stack,
+                   const int32_t *row_adapter, const int32_t *order, float *t, int ldt) {
+  // windows of 16 rows fill the matrix instruction; below 256 of them (one per compute unit) smaller ones are faster
+  int window = 16;
+  while (window > 1 && (N + window - 1) / window < 256) window /= 2;
+  const int nb = stack.max_rank <= 16 ? 1 : 2;
+  const dim3 grid((N + window - 1) / window, (stack.max_rank + 16 * nb - 1) / (16 * nb));
+  if (nb == 1)
+    narrow_kernel<1, 8, VEC><<<grid, 512, 0, st>>>(x, ldx, N, K, side, ldside, stack, row_adapter, order, window, t, ldt);
+  else
+    narrow_kernel<2, 8, VEC><<<grid, 512, 0, st>>>(x, ldx, N, K, side, ldside, stack, row_adapter, order, window, t, ldt);
+}
+
+template <int MB, int NB, bool NN, bool VEC>
+void launch_wide_tile(hipStream_t st, WideArgs p) {
+  p.tiles_m = (p.N + 16 * MB - 1) / (16 * MB);
+  p.tiles_n = (p.C + 16 * NB - 1) / (16 * NB);
+  const unsigned blocks = 8u * ((p.tiles_n + 7) / 8) * (unsigned)p.tiles_m;
+  wide_kernel<MB, NB, 8, NN, VEC><<<blocks, 512, 0, st>>>(p);
+}
+template <bool NN, bool VEC>
+void launch_wide(hipStream_t st, const WideArgs &p) {
+  const long long rows16 = (p.N + 15) / 16, cols16 = (p.C + 15) / 16;
+  if (rows16 * cols16 <= 256) launch_wide_tile<1, 1, NN, VEC>(st, p);
+  else if (rows16 * cols16 <= 1024) launch_wide_tile<1, 2, NN, VEC>(st, p);
+  else launch_wide_tile<2, 4, NN, VEC>(st, p);
+}
+
+int check_adapters(const khAdapters *ad, const int32_t *row_adapter, int32_t N, int32_t I, int32_t O) {
+  KH_REQUIRE(ad != nullptr && ad->num >= 0);
+  if (ad->num == 0) return KH_OK;
+  KH_REQUIRE(ad->max_rank >= 1 && ad->rows >= 0);
+  if (ad->max_rank > KH_MAX_ADAPTER_RANK) {
+    snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "adapters of rank %d: at most %d", ad->max_rank,
+             KH_MAX_ADAPTER_RANK);
+    return KH_ERR_TOO_LARGE;
+  }
+  KH_REQUIRE(ad->begin != nullptr && row_adapter != nullptr);
+  KH_REQUIRE(ad->rows == 0 || (ad->down != nullptr && ad->up != nullptr));
+  KH_REQUIRE(ad->lddown >= I && ad->ldup >= O);
+  return KH_OK;
+}
+
+// the library works on the device that hipK_init chose
+int check_device() {
+  int now = -1;
+  KH_HIP(hipGetDevice(&now));
+  KH_REQUIRE(now == kh::ctx().device);
+  return KH_OK;
+}
+
+}  // namespace
+
+KH_EXPORT int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int32_t num, int32_t *order,
+                                  int32_t *row_begin) {
+  KH_REQUIRE(N >= 0 && num >= 0 && row_begin != nullptr);
+  KH_REQUIRE(N == 0 || (row_adapter != nullptr && order != nullptr));
+  KH_CHECK_INIT();
+  int rc = check_device();
+  if (rc != KH_OK) return rc;
+  const int threads = N <= 256 ? 256 : 1024;
+  plan_kernel<<<(unsigned)num + 1u, threads, 0, kh::pick(s)>>>(row_adapter, N, num, order, row_begin);
+  return kh::launch_status();
+}
+
+KH_EXPORT int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, int32_t I, const float *in, int32_t ldin,
+                                   const float *W, int32_t ldw, const float *bias, const khAdapters *ad,
+                                   const int32_t *row_adapter, const int32_t *order, float *t, int32_t ldt, float *out,
+                                   int32_t ldout) {
+  KH_REQUIRE(act == KH_ACT_NONE || act == KH_ACT_SIGMOID || act == KH_ACT_SOFTMAX);
+  KH_REQUIRE(N >= 0 && O >= 0 && I >= 0);
+  int rc = check_adapters(ad, row_adapter, N, I, O);
+  if (rc != KH_OK) return rc;
+  KH_REQUIRE(ldin >= I && ldw >= I && ldout >= O);
+  KH_REQUIRE(ad->num == 0 || N == 0 || (t != nullptr && ldt >= ad->max_rank));
+  KH_REQUIRE(N == 0 || O == 0 || (out != nullptr && out != in && (I == 0 || (in != nullptr && W != nullptr))));
+  KH_CHECK_INIT();
+  rc = check_device();
+  if (rc != KH_OK) return rc;
+  if (N == 0 || O == 0) return KH_OK;
+  hipStream_t st = kh::pick(s);
+  const Stack stack = stack_of(*ad);
+  const bool vec = vec_ok(in, ldin) && vec_ok(W, ldw) && (ad->num == 0 || (vec_ok(ad->down, ad->lddown) &&
+                   vec_ok(ad->up, ad->ldup) && vec_ok(t, ldt)));
+  if (ad->num > 0) {
+    if (vec) launch_narrow<true>(st, in, ldin, N, I, ad->down, ad->lddown, stack, row_adapter, order, t, ldt);
+    else launch_narrow<false>(st, in, ldin, N, I, ad->down, ad->lddown, stack, row_adapter, order, t, ldt);
+    rc = kh::launch_status();
+    if (rc != KH_OK) return rc;
+  }
+  WideArgs p = {in, ldin, W, ldw, N, I, O, bias, ad->num > 0 ? t : nullptr, ldt, ad->up, ad->ldup, stack, row_adapter, order,
+                nullptr, 0, act, out, ldout, 0, 0};
+  if (vec) launch_wide<false, true>(st, p);
+  else launch_wide<false, false>(st, p);
+  rc = kh::launch_status();
+  if (rc != KH_OK || act != KH_ACT_SOFTMAX) return rc;
+  const MatrixDim d = {N, O, ldout};
+  return hipF_softmax(s, out, out, d);
+}
+
+KH_EXPORT int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t I, const float *e, int32_t lde,
+                                    const float *in, int32_t ldin, const float *W, int32_t ldw, const khAdapters *ad,
+                                    const int32_t *row_adapter, const int32_t *order, const int32_t *row_begin,
+                                    const float *t, int32_t ldt, float *u, int32_t ldu, const float *y, int32_t ldy,
+                                    float *eout, int32_t ldeout, float *gdown, int32_t ldgdown, float *gup,
+                                    int32_t ldgup) {
+  KH_REQUIRE(N >= 0 && O >= 0 && I >= 0);
+  int rc = check_adapters(ad, row_adapter, N, I, O);
+  if (rc != KH_OK) return rc;
+  const bool grads = ad->num > 0 && (gdown != nullptr || gup != nullptr);
+  KH_REQUIRE(N == 0 || O == 0 || (e != nullptr && lde >= O));
+  KH_REQUIRE(eout == nullptr || (W != nullptr && ldw >= I && ldeout >= I && eout != e && eout != in));
+  KH_REQUIRE(eout == nullptr || y == nullptr || ldy >= I);
+  KH_REQUIRE(ad->num == 0 || N == 0 || (u != nullptr && ldu >= ad->max_rank && u != t));
+  KH_REQUIRE(!grads || (row_begin != nullptr && (N == 0 || order != nullptr)));
+  KH_REQUIRE(gdown == nullptr || (ldgdown >= I && (N == 0 || (in != nullptr && ldin >= I))));
+  KH_REQUIRE(gup == nullptr || (ldgup >= O && (N == 0 || (t != nullptr && ldt >= ad->max_rank))));
+  KH_CHECK_INIT();
+  rc = check_device();
+  if (rc != KH_OK) return rc;
+  hipStream_t st = kh::pick(s);
+  const Stack stack = stack_of(*ad);
+  if (ad->num > 0 && N > 0) {
+    if (vec_ok(e, lde) && vec_ok(ad->up, ad->ldup))
+      launch_narrow<true>(st, e, lde, N, O, ad->up, ad->ldup, stack, row_adapter, order, u, ldu);
+    else launch_narrow<false>(st, e, lde, N, O, ad->up, ad->ldup, stack, row_adapter, order, u, ldu);
+    rc = kh::launch_status();
+    if (rc != KH_OK) return rc;
+  }
+  if (eout != nullptr && N > 0 && I > 0) {
+    WideArgs p = {e, lde, W, ldw, N, O, I, nullptr, ad->num > 0 ? u : nullptr, ldu, ad->down, ad->lddown, stack, row_adapter,
+                  order, y, ldy, KH_ACT_NONE, eout, ldeout, 0, 0};
+    const bool vec = vec_ok(e, lde) && vec_ok(W, ldw) && (ad->num == 0 || (vec_ok(ad->down, ad->lddown) && vec_ok(u, ldu)));
+    if (vec) launch_wide<true, true>(st, p);
+    else launch_wide<true, false>(st, p);
+    rc = kh::launch_status();
+    if (rc != KH_OK) return rc;
+  }
+  if (!grads || ad->rows == 0) return KH_OK;
+  const int rank_blocks = (ad->max_rank + 15) / 16;
+  GradArgs gd = {u, ldu, in, ldin, gdown != nullptr ? I : 0, gdown, ldgdown};
+  GradArgs gu = {t, ldt, e, lde, gup != nullptr ? O : 0, gup, ldgup};
+  const int cols = std::max(gd.C, gu.C);
+  if (cols == 0) return KH_OK;
+  const int col_tiles = (cols + 63) / 64;
+  if ((long long)col_tiles * ad->num > 0x7fffffffLL) {
+    snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "gradients of %d adapters of %d columns: too many", ad->num, cols);
+    return KH_ERR_TOO_LARGE;
+  }
+  const dim3 grid((unsigned)col_tiles * ad->num, 2 * rank_blocks);
+  const bool vec = (gdown == nullptr || vec_ok(in, ldin)) && (gup == nullptr || vec_ok(e, lde));
+  if (vec) grad_kernel<4, 8, true><<<grid, 512, 0, st>>>(gd, gu, N, stack, order, row_begin, col_tiles, rank_blocks);
+  else grad_kernel<4, 8, false><<<grid, 512, 0, st>>>(gd, gu, N, stack, order, row_begin, col_tiles, rank_blocks);
+  return kh::launch_status();
+}

@@ -17,6 +17,7 @@ HEADER_PATH = os.path.join(ROOT, "include", "kaldi_hip.h")
 NO_TRANS, TRANS = 111, 112
 ACT_NONE, ACT_SIGMOID, ACT_SOFTMAX = 0, 1, 2
 COMM_ID_BYTES = 128
+MAX_ADAPTER_RANK, MAX_TOP = 128, 128
 
 
 class MatrixDim(ctypes.Structure):
@@ -50,6 +51,13 @@ class SgdSegment(ctypes.Structure):
     """khSgdSegment: one run of elements of hipF_sgd_apply_segments with its hyper-parameters."""
     _fields_ = [("begin", ctypes.c_size_t), ("end", ctypes.c_size_t), ("gscale", ctypes.c_float),
                 ("momentum", ctypes.c_float), ("lr", ctypes.c_float), ("l2", ctypes.c_float)]
+
+
+class Adapters(ctypes.Structure):
+    """khAdapters: the adapters of one layer (device addresses; the memory behind them stays the caller's)."""
+    _fields_ = [("num", ctypes.c_int32), ("max_rank", ctypes.c_int32), ("rows", ctypes.c_int32), ("begin", ctypes.c_void_p),
+                ("scale", ctypes.c_void_p), ("down", ctypes.c_void_p), ("lddown", ctypes.c_int32), ("up", ctypes.c_void_p),
+                ("ldup", ctypes.c_int32)]
 
 
 _CTYPES = {
