@@ -382,6 +382,235 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
   }
 }
 
+// ---- the wide product, tiles through LDS ----------------------------------------------------------------------------
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 v4b __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ v16f mfma6_32(const Frag &a, const Frag &b, v16f c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.lo, b.hi, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.lo, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.mid, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.hi, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.mid, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.hi, c, 0, 0, 0);
+  return c;
+}
+
+// four floats as three times four bfloat16
+__device__ __forceinline__ void split4(v4f x, v4b &hi, v4b &mid, v4b &lo) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const v2f v = {x[i], x[i + 1]};
+    const v2b h = __builtin_convertvector(v, v2b);
+    const v2f r = {v.x - (float)h.x, v.y - (float)h.y};
+    const v2b m = __builtin_convertvector(r, v2b);
+    const v2f q = {r.x - (float)m.x, r.y - (float)m.y};
+    const v2b l = __builtin_convertvector(q, v2b);
+    hi[i] = h.x, hi[i + 1] = h.y;
+    mid[i] = m.x, mid[i + 1] = m.y;
+    lo[i] = l.x, lo[i + 1] = l.y;
+  }
+}
+
+// A tile of X rows by 32 of the inner dimension lies in LDS as three images (hi, mid, lo), each of 32-row blocks of
+// 4 * 32 slots of 16 bytes: slot kc * 32 + (row ^ 4 kc) holds the eight bfloat16 k = 8 kc .. 8 kc + 7 of a row, which is
+// what a lane hands to the 32x32x16 instruction.  The exclusive-or spreads the four slots of a row over the banks, so
+// that neither the stores (eight lanes per row) nor the loads (32 rows) meet in one.
+__device__ __forceinline__ int slot_of(int row, int kc) { return (row >> 5) * 128 + kc * 32 + ((row & 31) ^ (4 * kc)); }
+
+// One workgroup of eight waves (WM x WN) per tile of BM x BN; a wave has MB x NB blocks of 32 x 32.  Every step of 32 of
+// the inner dimension is loaded into registers two steps ahead, split there and stored to the other half of LDS while
+// this step's products run; one barrier per step.
+template <int WM, int WN, int MB, int NB, bool NN, bool VEC>
+__global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
+  constexpr int BM = 32 * MB * WM, BN = 32 * NB * WN;
+  constexpr int A_SLOTS = BM * 4, B_SLOTS = BN * 4;
+  __shared__ v8b lds[2][3][A_SLOTS + B_SLOTS];
+  static_assert(WM * WN == 8 && BM % 64 == 0, "eight waves");
+  constexpr int AU = BM * 8 / 512;                          // units of four floats a thread stages of X
+  constexpr int BU = NN ? 0 : BN * 8 / 512;                 // of W, rows along the inner dimension
+  constexpr int BC = NN ? (BN * 4 + 511) / 512 : 0;         // of W, eight floats down a column each
+
+  // tiles in groups of four rows of tiles, the groups dealt to the dies in whole runs: a die's tiles share their operands
+  const int total = p.tiles_m * p.tiles_n, per = (total + 7) / 8;
+  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
+  const int group = id / (4 * p.tiles_n), in_group = min(4, p.tiles_m - 4 * group), rest = id - group * 4 * p.tiles_n;
+  const int m0 = (4 * group + rest % in_group) * BM, n0 = (rest / in_group) * BN;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = wave / WN, wn = wave % WN, l31 = lane & 31, half = lane >> 5;
+
+  const float *ar[AU];
+#pragma unroll
+  for (int u = 0; u < AU; ++u) ar[u] = p.x + (size_t)max(row_of(p.order, m0 + (tid >> 3) + 64 * u, p.N), 0) * p.ldx;
+  const float *br[BU > 0 ? BU : 1];
+#pragma unroll
+  for (int u = 0; u < BU; ++u) br[u] = p.w + (size_t)min(n0 + (tid >> 3) + 64 * u, p.C - 1) * p.ldw;
+  const int ka = (tid & 7) * 4;
+
+  v4f ra[AU], rb[BU > 0 ? BU : 1];
+  float rc[BC > 0 ? BC : 1][8];
+  auto load4 = [&](const float *row, int k) -> v4f {
+    if (VEC && k + 4 <= p.K) return *reinterpret_cast<const v4f *>(row + k);
+    v4f v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = k + i < p.K ? row[k + i] : 0.f;
+    return v;
+  };
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < AU; ++u) ra[u] = load4(ar[u], k0 + ka);
+#pragma unroll
+    for (int u = 0; u < BU; ++u) rb[u] = load4(br[u], k0 + ka);
+#pragma unroll
+    for (int u = 0; u < BC; ++u) {
+      const int n = min(n0 + (tid + 512 * u) % BN, p.C - 1), kc = (tid + 512 * u) / BN;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int k = k0 + 8 * kc + e;
+        rc[u][e] = kc < 4 && k < p.K ? p.w[(size_t)k * p.ldw + n] : 0.f;
+      }
+    }
+  };
+  auto put = [&](int buf) {
+    const int kc = ka >> 3, sub = ka & 4;
+#pragma unroll
+    for (int u = 0; u < AU; ++u) {
+      v4b h, m, l;
+      split4(ra[u], h, m, l);
+      const int s = slot_of((tid >> 3) + 64 * u, kc);
+      *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][0][s]) + sub) = h;
+      *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][1][s]) + sub) = m;
+      *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][2][s]) + sub) = l;
+    }
+#pragma unroll
+    for (int u = 0; u < BU; ++u) {
+      v4b h, m, l;
+      split4(rb[u], h, m, l);
+      const int s = A_SLOTS + slot_of((tid >> 3) + 64 * u, kc);
+      *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][0][s]) + sub) = h;
+      *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][1][s]) + sub) = m;
+      *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][2][s]) + sub) = l;
+    }
+#pragma unroll
+    for (int u = 0; u < BC; ++u) {
+      const int n = (tid + 512 * u) % BN, c = (tid + 512 * u) / BN;
+      if (c < 4) {
+        const Frag f = split8(rc[u]);
+        const int s = A_SLOTS + slot_of(n, c);
+        lds[buf][0][s] = f.hi, lds[buf][1][s] = f.mid, lds[buf][2][s] = f.lo;
+      }
+    }
+  };
+
+  v16f acc[MB][NB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
+
+  const int steps = (p.K + 31) / 32;
+  if (steps > 0) {
+    fetch(0);
+    put(0);
+    if (steps > 1) fetch(32);
+    __syncthreads();
+  }
+  for (int s = 0; s < steps; ++s) {
+    const int buf = s & 1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      Frag fa[MB], fb[NB];
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const int at = slot_of(32 * (wm * MB + m) + l31, 2 * h + half);
+        fa[m].hi = lds[buf][0][at], fa[m].mid = lds[buf][1][at], fa[m].lo = lds[buf][2][at];
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int at = A_SLOTS + slot_of(32 * (wn * NB + n) + l31, 2 * h + half);
+        fb[n].hi = lds[buf][0][at], fb[n].mid = lds[buf][1][at], fb[n].lo = lds[buf][2][at];
+      }
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[m][n] = mfma6_32(fa[m], fb[n], acc[m][n]);
+      if (h == 0 && s + 1 < steps) {
+        put(buf ^ 1);
+        if (s + 2 < steps) fetch(32 * (s + 2));
+      }
+    }
+    __syncthreads();
+  }
+
+  // the adapters' part, straight into registers: a wave goes through the runs of equal adapters in its rows
+  const int wave_m0 = m0 + 32 * MB * wm, wave_n0 = n0 + 32 * NB * wn;
+#pragma unroll
+  for (int m = 0; m < MB; ++m) {
+    const int row = lane < 32 ? row_of(p.order, wave_m0 + 32 * m + lane, p.N) : -1;
+    const int my_row = __shfl(row, l31, 64);
+    if (p.t) {
+      const int g = adapter_of(p.row_adapter, p.st.num, row);
+      const Runs runs = find_runs(g, lane);
+      const float *tr = p.t + (size_t)max(my_row, 0) * p.ldt;
+      for (unsigned long long left = runs.starts; left; left &= left - 1ull) {
+        const int s = __builtin_ctzll(left);
+        const unsigned mask = (unsigned)run_mask(runs, s);
+        int lo, rank;
+        stack_rows(p.st, __shfl(g, s, 64), &lo, &rank);
+        v16f d[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) d[n][i] = 0.f;
+        for (int k0 = 0; k0 < rank; k0 += 16) {
+          float a[8];
+          load_row8<VEC>(tr, k0 + 8 * half, rank, a);
+          const Frag fa = split8(a);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const int c = wave_n0 + 32 * n + l31;
+            float b[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int k = k0 + 8 * half + e;
+              b[e] = k < rank && c < p.C ? p.side[(size_t)(lo + k) * p.ldside + c] : 0.f;
+            }
+            d[n] = mfma6_32(fa, split8(b), d[n]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if ((mask >> (8 * (i >> 2) + 4 * half + (i & 3))) & 1u) acc[m][n][i] += d[n][i];
+      }
+    }
+    // out: lane l31 has a column, i counts rows
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = __shfl(row, 8 * (i >> 2) + 4 * half + (i & 3), 64);
+      if (r < 0) continue;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int c = wave_n0 + 32 * n + l31;
+        if (c >= p.C) continue;
+        float v = acc[m][n][i];
+        if (p.bias) v += p.bias[c];
+        if (p.act == KH_ACT_SIGMOID) v = kh::sigmoidf(v);
+        if (p.y) {
+          const float yv = p.y[(size_t)r * p.ldy + c];
+          v = v * yv * (1.f - yv);
+        }
+        p.out[(size_t)r * p.ldout + c] = v;
+      }
+    }
+  }
+}
+
 // ---- gradients of the stacks ----------------------------------------------------------------------------------------
 // g_side[begin + k, c] = sum over the rows r of an adapter of narrow[r, k] * wide[r, c].  One workgroup per adapter,
 // block of 16 * NB columns and block of 16 rank rows; its waves take steps of 32 rows in turn.
@@ -467,8 +696,16 @@ void launch_wide_tile(hipStream_t st, WideArgs p) {
   const unsigned blocks = 8u * ((p.tiles_n + 7) / 8) * (unsigned)p.tiles_m;
   wide_kernel<MB, NB, 8, NN, VEC><<<blocks, 512, 0, st>>>(p);
 }
+template <int WM, int WN, int MB, int NB, bool NN, bool VEC>
+void launch_tiled(hipStream_t st, WideArgs p) {
+  p.tiles_m = (p.N + 32 * MB * WM - 1) / (32 * MB * WM);
+  p.tiles_n = (p.C + 32 * NB * WN - 1) / (32 * NB * WN);
+  const unsigned blocks = 8u * (((unsigned)p.tiles_m * p.tiles_n + 7) / 8);
+  tiled_kernel<WM, WN, MB, NB, NN, VEC><<<blocks, 512, 0, st>>>(p);
+}
 template <bool NN, bool VEC>
 void launch_wide(hipStream_t st, const WideArgs &p) {
+  if (p.N >= 1024) return launch_tiled<4, 2, 2, 2, NN, VEC>(st, p);
   const long long rows16 = (p.N + 15) / 16, cols16 = (p.C + 15) / 16;
   if (rows16 * cols16 <= 256) launch_wide_tile<1, 1, NN, VEC>(st, p);
   else if (rows16 * cols16 <= 1024) launch_wide_tile<1, 2, NN, VEC>(st, p);
