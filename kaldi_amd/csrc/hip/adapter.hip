@@ -451,26 +451,39 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
 
   v4f ra[AU], rb[BU > 0 ? BU : 1];
   float rc[BC > 0 ? BC : 1][8];
-  auto load4 = [&](const float *row, int k) -> v4f {
-    if (VEC && k + 4 <= p.K) return *reinterpret_cast<const v4f *>(row + k);
-    v4f v;
+  const float *bc[BC > 0 ? BC : 1];  // column n of W, from row 8 kc
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = k + i < p.K ? row[k + i] : 0.f;
-    return v;
-  };
-  auto fetch = [&](int k0) {
+  for (int u = 0; u < BC; ++u)
+    bc[u] = p.w + (size_t)(8 * ((tid + 512 * u) / BN)) * p.ldw + min(n0 + (tid + 512 * u) % BN, p.C - 1);
+  // the step at k0 into registers: a whole one, or what is left of K (zeros behind it)
+  auto fetch_whole = [&](int k0) {
 #pragma unroll
-    for (int u = 0; u < AU; ++u) ra[u] = load4(ar[u], k0 + ka);
+    for (int u = 0; u < AU; ++u) ra[u] = *reinterpret_cast<const v4f *>(ar[u] + k0 + ka);
 #pragma unroll
-    for (int u = 0; u < BU; ++u) rb[u] = load4(br[u], k0 + ka);
+    for (int u = 0; u < BU; ++u) rb[u] = *reinterpret_cast<const v4f *>(br[u] + k0 + ka);
 #pragma unroll
     for (int u = 0; u < BC; ++u) {
-      const int n = min(n0 + (tid + 512 * u) % BN, p.C - 1), kc = (tid + 512 * u) / BN;
+      if (BC * 512 > BN * 4 && (tid + 512 * u) / BN >= 4) continue;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int k = k0 + 8 * kc + e;
-        rc[u][e] = kc < 4 && k < p.K ? p.w[(size_t)k * p.ldw + n] : 0.f;
-      }
+      for (int e = 0; e < 8; ++e) rc[u][e] = bc[u][(size_t)(k0 + e) * p.ldw];
+    }
+  };
+  auto fetch = [&](int k0) {
+    if (VEC && k0 + 32 <= p.K) return fetch_whole(k0);
+#pragma unroll
+    for (int u = 0; u < AU; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ra[u][i] = k0 + ka + i < p.K ? ar[u][k0 + ka + i] : 0.f;
+#pragma unroll
+    for (int u = 0; u < BU; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rb[u][i] = k0 + ka + i < p.K ? br[u][k0 + ka + i] : 0.f;
+#pragma unroll
+    for (int u = 0; u < BC; ++u) {
+      const int kc = (tid + 512 * u) / BN;
+      if (BC * 512 > BN * 4 && kc >= 4) continue;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) rc[u][e] = k0 + 8 * kc + e < p.K ? bc[u][(size_t)(k0 + e) * p.ldw] : 0.f;
     }
   };
   auto put = [&](int buf) {
@@ -513,36 +526,49 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
       for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
 
   const int steps = (p.K + 31) / 32;
+  // the products of one half of a step: the six part products in turn, each over all blocks (a block's sum is then
+  // not waited for)
+  auto multiply = [&](int buf, int h) {
+    v8b fa[MB][3], fb[NB][3];
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) fa[m][i] = lds[buf][i][slot_of(32 * (wm * MB + m) + l31, 2 * h + half)];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) fb[n][i] = lds[buf][i][A_SLOTS + slot_of(32 * (wn * NB + n) + l31, 2 * h + half)];
+    constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+    for (int q = 0; q < 6; ++q)
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+          acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[m][pa[q]], fb[n][pb[q]], acc[m][n], 0, 0, 0);
+  };
   if (steps > 0) {
     fetch(0);
     put(0);
     if (steps > 1) fetch(32);
     __syncthreads();
   }
-  for (int s = 0; s < steps; ++s) {
-    const int buf = s & 1;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      Frag fa[MB], fb[NB];
-#pragma unroll
-      for (int m = 0; m < MB; ++m) {
-        const int at = slot_of(32 * (wm * MB + m) + l31, 2 * h + half);
-        fa[m].hi = lds[buf][0][at], fa[m].mid = lds[buf][1][at], fa[m].lo = lds[buf][2][at];
-      }
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int at = A_SLOTS + slot_of(32 * (wn * NB + n) + l31, 2 * h + half);
-        fb[n].hi = lds[buf][0][at], fb[n].mid = lds[buf][1][at], fb[n].lo = lds[buf][2][at];
-      }
-#pragma unroll
-      for (int m = 0; m < MB; ++m)
-#pragma unroll
-        for (int n = 0; n < NB; ++n) acc[m][n] = mfma6_32(fa[m], fb[n], acc[m][n]);
-      if (h == 0 && s + 1 < steps) {
-        put(buf ^ 1);
-        if (s + 2 < steps) fetch(32 * (s + 2));
-      }
+  int s = 0;
+  if (VEC)
+    for (; 32 * (s + 3) <= p.K; ++s) {
+      const int buf = s & 1;
+      multiply(buf, 0);
+      put(buf ^ 1);
+      fetch_whole(32 * (s + 2));
+      multiply(buf, 1);
+      __syncthreads();
     }
+  for (; s < steps; ++s) {
+    const int buf = s & 1;
+    multiply(buf, 0);
+    if (s + 1 < steps) put(buf ^ 1);
+    if (s + 2 < steps) fetch(32 * (s + 2));
+    multiply(buf, 1);
     __syncthreads();
   }
 
