@@ -37,27 +37,61 @@ template <int THREADS, bool VEC>
 __device__ __forceinline__ int column_of(int c0, int tid, int i) {
   return VEC ? c0 + ((i >> 2) * THREADS + tid) * 4 + (i & 3) : c0 + i * THREADS + tid;
 }
+// A chunk's `left` columns from `from` on (what a thread gets behind the row's end is some other column of it: end_chunk
+// makes it -inf).  Loads are not guarded one by one but moved back to the row's last 16 bytes, which begin inside the row:
+// an aligned load that begins inside an allocation stays in its page.
 template <int THREADS, bool VEC>
-__device__ __forceinline__ void load_chunk(const float *row, int c0, int C, int tid, float (&z)[kHold]) {
+__device__ __forceinline__ void load_chunk(const float *from, unsigned left, int tid, float (&z)[kHold]) {
   if (VEC) {
 #pragma unroll
     for (int i = 0; i < kHold; i += 4) {
-      const int c = column_of<THREADS, VEC>(c0, tid, i);
-      if (c + 4 <= C) {
-        const v4f v = *reinterpret_cast<const v4f *>(row + c);
-        z[i] = v.x, z[i + 1] = v.y, z[i + 2] = v.z, z[i + 3] = v.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) z[i + j] = c + j < C ? row[c + j] : -INFINITY;
-      }
+      const unsigned c = ((i >> 2) * THREADS + tid) * 4;
+      const v4f v = *reinterpret_cast<const v4f *>(from + min(c, (left - 1u) & ~3u));
+      z[i] = v.x, z[i + 1] = v.y, z[i + 2] = v.z, z[i + 3] = v.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) {
-      const int c = column_of<THREADS, VEC>(c0, tid, i);
-      z[i] = c < C ? row[c] : -INFINITY;
-    }
+    for (int i = 0; i < kHold; ++i) z[i] = from[min((unsigned)(i * THREADS + tid), left - 1u)];
   }
+}
+template <int THREADS, bool VEC>
+__device__ __forceinline__ void end_chunk(unsigned left, int tid, float (&z)[kHold]) {
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int w = VEC ? 4 : 1;
+#pragma unroll
+  for (int i = 0; i < kHold; i += w)
+    if (left < (unsigned)((i / w) * THREADS + 64 * wave + 64) * w)  // (a wave whose columns are all there has nothing to do)
+#pragma unroll
+      for (int j = 0; j < w; ++j)
+        if (column_of<THREADS, VEC>(0, tid, i + j) >= (int)left) z[i + j] = -INFINITY;
+}
+
+// Reductions over a wave in six steps of cross-lane operands (within rows of 16 lanes, then from row to row); every lane
+// gets the result, as a scalar.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float lanes(float otherwise, float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(otherwise), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float last_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ float wave_add(float v) {
+  v += lanes<0x111, 0xf>(0.f, v);  // row_shr:1, 2, 4, 8
+  v += lanes<0x112, 0xf>(0.f, v);
+  v += lanes<0x114, 0xf>(0.f, v);
+  v += lanes<0x118, 0xf>(0.f, v);
+  v += lanes<0x142, 0xa>(0.f, v);  // row_bcast:15, 31
+  v += lanes<0x143, 0xc>(0.f, v);
+  return last_lane(v);
+}
+__device__ __forceinline__ float wave_most(float v) {  // (passes over NaN, as fmaxf does)
+  v = fmaxf(v, lanes<0x111, 0xf>(-INFINITY, v));
+  v = fmaxf(v, lanes<0x112, 0xf>(-INFINITY, v));
+  v = fmaxf(v, lanes<0x114, 0xf>(-INFINITY, v));
+  v = fmaxf(v, lanes<0x118, 0xf>(-INFINITY, v));
+  v = fmaxf(v, lanes<0x142, 0xa>(-INFINITY, v));
+  v = fmaxf(v, lanes<0x143, 0xc>(-INFINITY, v));
+  return last_lane(v);
 }
 
 template <int THREADS>
@@ -73,148 +107,230 @@ __device__ __forceinline__ float all_max(float v, float *red) {
 }
 
 // ---- the K largest of a row -------------------------------------------------------------------------------------------
-// Order of the answer: by value, NaN above everything, -0 = +0, then by ascending column.  A 64-bit key has it: the
-// float's bits made monotone in the upper half, the complement of the column in the lower.
+// Order of the answer: by value, NaN above everything, -0 = +0, then by ascending column.  ordered() makes the float's
+// bits monotone; a 64-bit key with the complement of the column below them has the whole order.
 typedef unsigned long long key_t;
 __device__ __forceinline__ unsigned ordered(float x) {
-  if (x != x) return 0xffffffffu;
   const unsigned b = __float_as_uint(x + 0.f);  // -0 + 0 = +0
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const unsigned u = b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+  return x != x ? 0xffffffffu : u;
+}
+__device__ __forceinline__ float unordered(unsigned u) {
+  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
 }
 __device__ __forceinline__ key_t key_of(float x, int c) { return (key_t)ordered(x) << 32 | (unsigned)~c; }
 
-constexpr int kCap = 1024;  // candidates of a chunk, next to the KH_MAX_TOP of the chunks before
+constexpr int kCap = 1024;   // candidates of a chunk, next to the KH_MAX_TOP of the chunks before
+constexpr int kTopWaves = 6;  // waves per SIMD (at most 80 registers: three workgroups of 512 threads on a compute unit)
 
-// One workgroup per row, chunk by chunk.  A chunk's threads form G >= K groups; the K-th largest of the groups' maxima is
-// a lower bound of the chunk's K-th largest, which leaves few more than K candidates where large values are spread over
-// the row.  Candidates (also above the K-th of the chunks before) are collected in LDS and ranked by counting; the K
-// largest are kept.  Where more than kCap pass (large values crowded into few groups) the bound is raised by bisection
-// on the keys, which are distinct.
+// 16 (VEC) or 4 bytes per lane straight into LDS: lane l's land at `to` + l * size, `to` the same for the whole wave
+template <bool VEC>
+__device__ __forceinline__ void load_to_lds(const float *from, float *to) {
+  typedef __attribute__((address_space(1))) const void gvoid;
+  typedef __attribute__((address_space(3))) void lvoid;
+  if constexpr (VEC) __builtin_amdgcn_global_load_lds((gvoid *)from, (lvoid *)to, 16, 0, 0);
+  else __builtin_amdgcn_global_load_lds((gvoid *)from, (lvoid *)to, 4, 0, 0);
+}
+
+// A workgroup takes one row after another, chunk by chunk, and has the next chunk (of this row or the next) loaded into LDS
+// while it works on one in registers; a wave waits for its own part only.  4096 rows of 9000: 44 us, 3.4 TB/s (a plain
+// sum of as much memory reads at 4.0; one row per workgroup without the look-ahead: 106 us); 256 rows of 70001: 28 us.
+// A row's first chunk: its threads form G groups; a value that at least K groups' maxima reach is a lower bound of the
+// chunk's K-th largest, and where large values are spread over the row few more than K elements reach the best such value.
+// It is found by bisection to K .. 1.25 K groups, every wave for itself.  (Later chunks: the K-th largest so far.)  The
+// elements that reach the bound are collected in LDS and ranked by counting; the K largest are kept.  Where more than kCap reach the bound (large values crowded into few groups, many equal ones), and
+// where the chunk holds a NaN or +inf, a bound on the distinct keys is found by bisection over the chunk.
 template <int THREADS, bool VEC>
-__global__ __launch_bounds__(THREADS) void row_top_kernel(const float *mat, MatrixDim d, int K, int32_t *idx, int ldidx,
+__global__ __launch_bounds__(THREADS, kTopWaves) void row_top_kernel(const float *mat, MatrixDim d, int K, int32_t *idx, int ldidx,
                                                           float *val, int ldval, float *lse) {
-  constexpr int G = THREADS < 256 ? THREADS : 256;  // groups: one per thread, or 256
-  __shared__ key_t cand[kCap + KH_MAX_TOP];
+  constexpr int G = THREADS < 256 ? THREADS : 256, per = THREADS / G, waves = THREADS / 64, chunk = THREADS * kHold;
+  __shared__ __align__(16) float ahead[chunk];
+  __shared__ __align__(16) key_t cand[kCap + KH_MAX_TOP];
   __shared__ key_t best[KH_MAX_TOP];
-  __shared__ key_t gmax[G];
-  __shared__ key_t bound_s;
+  __shared__ float gmax[G];
+  __shared__ float part_s[waves];
   __shared__ int count_s;
-  __shared__ float red[16];
-  const int tid = threadIdx.x;
-  const float *row = mat + (size_t)blockIdx.x * d.stride;
-  int have = 0;         // valid entries of best[]
-  float m = -INFINITY;  // running maximum and sum of exp(x - m)
-  float sum = 0.f;
-  const ExpScale one = {1.44269502f, 1.92596303e-8f};
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  for (int c0 = 0; c0 < d.cols; c0 += THREADS * kHold) {
-    float z[kHold];
-    load_chunk<THREADS, VEC>(row, c0, d.cols, tid, z);
-    if (lse) {
-      float cm = z[0];
+  // (what lies behind the row's end is some other column of it here, and becomes -inf below)
+  auto load = [&](const float *from, int cols) {
+    const unsigned last = VEC ? (unsigned)(cols - 1) & ~3u : (unsigned)(cols - 1);
+    constexpr int w = VEC ? 4 : 1;
 #pragma unroll
-      for (int i = 1; i < kHold; ++i) cm = fmaxf(cm, z[i]);
-      cm = fmaxf(m, all_max<THREADS>(cm, red));
-      // (a NaN in a chunk of -inf: m stays -inf, and the sum takes the NaN)
-      const float base = cm == -INFINITY ? 0.f : cm;
+    for (int i = 0; i < kHold / w; ++i)
+      load_to_lds<VEC>(from + min((unsigned)(i * THREADS + tid) * w, last), ahead + (i * THREADS + wave * 64) * w);
+  };
+  if (blockIdx.x < (unsigned)d.rows && d.cols > 0) load(mat + (size_t)blockIdx.x * d.stride, d.cols);
+  for (long long r = blockIdx.x; r < d.rows; r += gridDim.x) {
+    const float *row = mat + (size_t)r * d.stride;
+    int have = 0;          // valid entries of best[]
+    float m = -INFINITY;   // running maximum and sum of exp(x - m)
+    float sum = 0.f;
+    for (int c0 = 0; c0 < d.cols; c0 += chunk) {
+      float z[kHold];
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part has arrived
+#pragma unroll
+      for (int i = 0; i < kHold; ++i) z[i] = ahead[column_of<THREADS, VEC>(0, tid, i)];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and has been read: the next may come
+      const int left = d.cols - c0;
+      if (left > chunk) load(row + c0 + chunk, left - chunk);
+      else if (r + gridDim.x < d.rows) load(row + (size_t)gridDim.x * d.stride, d.cols);
+      int t = tid;  // (columns are worked out where they are needed: hidden from the compiler, which would keep 20 of them)
+      asm volatile("" : "+v"(t));
+      end_chunk<THREADS, VEC>(left, t, z);
+      float mine = z[0];
+#pragma unroll
+      for (int i = 1; i < kHold; ++i) mine = fmaxf(mine, z[i]);
+#pragma unroll
+      for (int o = per / 2; o > 0; o >>= 1) mine = fmaxf(mine, __shfl_xor(mine, o, 64));
+      if (tid % per == 0) gmax[tid / per] = mine;
+      if (tid == 0) count_s = have;
+      __syncthreads();
+      float g[G / 64];
+#pragma unroll
+      for (int j = 0; j < G / 64; ++j) g[j] = gmax[lane + 64 * j];
+      float most = g[0], least = g[0];
+#pragma unroll
+      for (int j = 1; j < G / 64; ++j) most = fmaxf(most, g[j]), least = fminf(least, g[j]);
+      most = wave_most(most);
+      const float top = fmaxf(m, most);
+      const float base = top == -INFINITY ? 0.f : top;
+      // the sum; also what tells of a NaN or +inf
       float part = 0.f;
 #pragma unroll
-      for (int i = 0; i < kHold; ++i) part += exp_scaled(z[i] - base, one);
-      part = all_sum<THREADS>(part, red);
-      sum = (sum == 0.f ? 0.f : sum * expf(m - base)) + part;
-      m = cm;
-    }
-    // the thread's largest, then the group's
-    key_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < kHold; ++i) {
-      const int c = column_of<THREADS, VEC>(c0, tid, i);
-      const key_t k = key_of(z[i], c);
-      if (c < d.cols && k > mine) mine = k;
-    }
-    constexpr int per = THREADS / G;
-#pragma unroll
-    for (int o = per / 2; o > 0; o >>= 1) {
-      const key_t other = __shfl_xor(mine, o, 64);
-      mine = other > mine ? other : mine;
-    }
-    __syncthreads();  // (the chunk before is done with the shared arrays)
-    if (tid % per == 0) gmax[tid / per] = mine;
-    if (tid == 0) {
-      count_s = 0;
-      bound_s = have == K ? best[K - 1] : 0;
-    }
-    __syncthreads();
-    // The K-th largest of the groups' maxima, by counting; empty groups hold 0, which bounds nothing.  K > G (64
-    // threads): no bound from here.
-    if (tid < G && K <= G) {
-      const key_t k = gmax[tid];
-      int above = 0;
-      for (int j = 0; j < G; ++j) above += gmax[j] > k;
-      if (above == K - 1 && k > bound_s) bound_s = k;  // keys are distinct but for 0: one thread writes, or all a 0
-    }
-    __syncthreads();
-    // Candidates: this chunk's keys from the bound on.  `lo` lets too many through or is the answer, `hi` too few; keys are
-    // distinct, so the two cannot meet with more than kCap >= K + 1 between them: at most 64 rounds.
-    key_t lo = bound_s, hi = ~0ull, try_at = lo;
-    for (int round = 0; round <= 64; ++round) {
+      for (int i = 0; i < kHold; ++i) part += __builtin_amdgcn_exp2f((z[i] - base) * 1.44269504088896340736f);
+      part = wave_add(part);
+      if (lane == 0) part_s[wave] = part;
+      sum = sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f((m - base) * 1.44269504088896340736f);
+      m = top;
+      float bound = have == K ? unordered((unsigned)(best[K - 1] >> 32)) : -INFINITY;
+      if (tid < have) cand[tid] = best[tid];
+      __syncthreads();
+      float here = 0.f;
+      for (int w = 0; w < waves; ++w) here += part_s[w];
+      sum += here;
+      bool odd = here != here;  // (the same for all threads)
       int n = 0;
+      // Collect with the K-th largest of the chunks before as the bound; in the first chunk, and where that lets too many
+      // through, with the groups'.
+      for (int attempt = have == K ? 0 : 1; attempt < 2 && !odd; ++attempt) {
+        if (attempt) {
+          // `low` is reached by at least K groups (K <= G), `high` by fewer, or it is the largest of all.  What is behind
+          // the row's end counts as -inf: no bound is the worse for it.
+          unsigned low = ordered(-wave_most(-least)), high = ordered(most);
+          for (int round = 0; round < 32 && high - low > 1u; ++round) {
+            const unsigned mid = low + (high - low) / 2;
+            const float at = unordered(mid);
+            int reach = 0;
 #pragma unroll
-      for (int i = 0; i < kHold; ++i) {
-        const int c = column_of<THREADS, VEC>(c0, tid, i);
-        n += c < d.cols && key_of(z[i], c) >= try_at;
+            for (int j = 0; j < G / 64; ++j) reach += __popcll(__ballot(g[j] >= at));
+            if (reach >= K) {
+              low = mid;
+              if (reach <= K + (K >> 2)) break;
+            } else {
+              high = mid;
+            }
+          }
+          bound = fmaxf(bound, unordered(low));
+          if (!(bound > -INFINITY)) {  // (it would let in what is behind the row's end)
+            odd = true;
+            break;
+          }
+        }
+        // one place in the list per wave, then places by counting
+        int hits = 0;
+#pragma unroll
+        for (int i = 0; i < kHold; ++i) hits += __popcll(__ballot(z[i] >= bound));
+        if (hits) {
+          int at = 0;
+          if (lane == 0) at = atomicAdd(&count_s, hits);
+          at = __builtin_amdgcn_readfirstlane(at);
+          float limit = bound;
+          asm volatile("" : "+v"(limit), "+v"(t));  // (compared anew: 20 masks would not fit the scalar registers)
+#pragma unroll
+          for (int i = 0; i < kHold; ++i) {
+            const unsigned long long hit = __ballot(z[i] >= limit);
+            if (hit) {
+              const int place = at + __builtin_amdgcn_mbcnt_hi((unsigned)(hit >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hit, 0));
+              float x = z[i];
+              asm volatile("" : "+v"(x));  // (its key is made here, for the few, not ahead for all)
+              if (x >= limit && place < kCap + KH_MAX_TOP) cand[place] = key_of(x, column_of<THREADS, VEC>(c0, t, i));
+              at += __popcll(hit);
+            }
+          }
+        }
+        __syncthreads();
+        n = count_s;
+        if (n <= kCap + have) break;
+        __syncthreads();  // (count_s has been read)
+        if (tid == 0) count_s = have;
+        __syncthreads();
       }
+      if (odd || n > kCap + have) {
+        // (rare: the chunk is read again, from the cache, instead of being kept in registers for this)
+        const int end = d.cols - c0 > chunk ? c0 + chunk : d.cols;
+        // `lo` lets too many through, `hi` too few: the keys between are distinct, so a bound that lets between K and
+        // kCap through is found within 64 rounds.  A chunk of at most kCap elements is taken whole.
+        key_t lo = 0, hi = ~0ull, found = end - c0 <= kCap ? 0 : hi;
+        for (int round = 0; round < 64 && found; ++round) {
+          const key_t try_at = lo + (hi - lo) / 2;
+          int reach = 0;
+          for (int c = c0 + tid; c < end; c += THREADS) reach += key_of(row[c], c) >= try_at;
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-      __syncthreads();  // (count_s of the round before has been read)
-      if (tid == 0) count_s = 0;
+          for (int o = 32; o > 0; o >>= 1) reach += __shfl_xor(reach, o, 64);
+          __syncthreads();  // (count_s has been read)
+          if (tid == 0) count_s = 0;
+          __syncthreads();
+          if (lane == 0) atomicAdd(&count_s, reach);
+          __syncthreads();
+          const int total = count_s;
+          if (total >= K && total <= kCap) {
+            found = try_at;
+            break;
+          }
+          if (total > kCap) lo = try_at;
+          else hi = try_at;
+        }
+        __syncthreads();
+        if (tid == 0) count_s = have;
+        __syncthreads();
+        for (int c = c0 + tid; c < end; c += THREADS) {
+          const key_t k = key_of(row[c], c);
+          if (k >= found) {
+            const int at = atomicAdd(&count_s, 1);
+            if (at < kCap + KH_MAX_TOP) cand[at] = k;
+          }
+        }
+        __syncthreads();
+        n = min(count_s, kCap + KH_MAX_TOP);
+      }
+      // a candidate's place is the number of larger ones: four lanes count for one candidate
+      for (int i0 = 0; i0 < n; i0 += THREADS / 4) {
+        const int i = i0 + (tid >> 2);
+        if (i >= n) break;
+        const key_t k = cand[i];
+        int above = 0;
+#pragma unroll 4
+        for (int j = tid & 3; j < n; j += 4) above += cand[j] > k;
+        above += __shfl_xor(above, 1, 64);
+        above += __shfl_xor(above, 2, 64);
+        if (above < K && (tid & 3) == 0) best[above] = k;
+      }
+      have = min(K, n);
       __syncthreads();
-      if ((tid & 63) == 0) atomicAdd(&count_s, n);
-      __syncthreads();
-      const int total = count_s;
-      if (total <= kCap && (round == 0 || total >= K)) {
-        lo = try_at;
-        break;
+    }
+    for (int k = tid; k < K; k += THREADS) {
+      int c = -1;
+      float v = -INFINITY;
+      if (k < have) {
+        c = (int)~(unsigned)best[k];
+        v = row[c];
       }
-      if (total > kCap) lo = try_at;
-      else hi = try_at;
-      try_at = lo + (hi - lo) / 2;
+      idx[(size_t)r * ldidx + k] = c;
+      val[(size_t)r * ldval + k] = v;
     }
-    __syncthreads();
-    if (tid == 0) count_s = have;
-    if (tid < have) cand[tid] = best[tid];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kHold; ++i) {
-      const int c = column_of<THREADS, VEC>(c0, tid, i);
-      const key_t k = key_of(z[i], c);
-      if (c < d.cols && k >= lo) {
-        const int at = atomicAdd(&count_s, 1);
-        if (at < kCap + KH_MAX_TOP) cand[at] = k;
-      }
-    }
-    __syncthreads();
-    const int n = min(count_s, kCap + KH_MAX_TOP);
-    for (int i = tid; i < n; i += THREADS) {
-      const key_t k = cand[i];
-      int above = 0;
-      for (int j = 0; j < n; ++j) above += cand[j] > k;
-      if (above < K) best[above] = k;
-    }
-    have = min(K, n);
-    __syncthreads();
+    if (lse && tid == 0) lse[r] = sum == 0.f ? -INFINITY : m + logf(sum);
   }
-  for (int k = tid; k < K; k += THREADS) {
-    int c = -1;
-    float v = -INFINITY;
-    if (k < have) {
-      c = (int)~(unsigned)best[k];
-      v = row[c];
-    }
-    idx[(size_t)blockIdx.x * ldidx + k] = c;
-    val[(size_t)blockIdx.x * ldval + k] = v;
-  }
-  if (lse && tid == 0) lse[blockIdx.x] = sum == 0.f ? -INFINITY : (float)((double)m + log((double)sum));
 }
 
 // ---- loss and gradient towards a teacher's logits ----------------------------------------------------------------------
@@ -263,7 +379,8 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs p) {
   float m = -INFINITY, sum_t = 0.f, sum_1 = 0.f;
   const bool single = C <= THREADS * kHold;
   for (int c0 = 0; c0 < C; c0 += THREADS * kHold) {
-    load_chunk<THREADS, VEC>(row, c0, C, tid, z);
+    load_chunk<THREADS, VEC>(row + c0, C - c0, tid, z);
+    end_chunk<THREADS, VEC>(C - c0, tid, z);
     float cm = z[0];
 #pragma unroll
     for (int i = 1; i < kHold; ++i) cm = fmaxf(cm, z[i]);
@@ -325,7 +442,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs p) {
   const float ft = some ? ws / sum_t : 0.f, f1 = labelled ? wh / sum_1 : 0.f;
   const float base = m == -INFINITY ? 0.f : m;
   for (int c0 = 0; c0 < C; c0 += THREADS * kHold) {
-    if (!single) load_chunk<THREADS, VEC>(row, c0, C, tid, z);
+    if (!single) load_chunk<THREADS, VEC>(row + c0, C - c0, tid, z);
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
       const float x = z[i] - base;
@@ -385,19 +502,23 @@ int check_device() {
   return KH_OK;
 }
 
+template <int THREADS, bool VEC>
+void launch_row_top_as(hipStream_t st, const float *mat, MatrixDim d, int K, int32_t *idx, int ldidx, float *val, int ldval,
+                       float *lse) {
+  // as many workgroups as run at once, each with its share of the rows
+  constexpr unsigned by_lds = 163840u / (THREADS * kHold * 4u + (kCap + 2 * KH_MAX_TOP) * 8u + 2048u);
+  constexpr unsigned by_waves = kTopWaves * 4u / (THREADS / 64);
+  const unsigned rows = (unsigned)d.rows, most = 256u * (by_lds < by_waves ? by_lds : by_waves);
+  row_top_kernel<THREADS, VEC><<<rows < most ? rows : most, THREADS, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
+}
 template <bool VEC>
 void launch_row_top(hipStream_t st, const float *mat, MatrixDim d, int K, int32_t *idx, int ldidx, float *val, int ldval,
                     float *lse) {
-  const unsigned rows = (unsigned)d.rows;
-  // the fewest threads that hold the row; K candidates need K groups
-  if (d.cols <= 64 * kHold && K <= 64)
-    row_top_kernel<64, VEC><<<rows, 64, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
-  else if (d.cols <= 256 * kHold)
-    row_top_kernel<256, VEC><<<rows, 256, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
-  else if (d.cols <= 512 * kHold)
-    row_top_kernel<512, VEC><<<rows, 512, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
-  else
-    row_top_kernel<1024, VEC><<<rows, 1024, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
+  // the fewest threads that hold the row
+  if (d.cols <= 64 * kHold && K <= 64) launch_row_top_as<64, VEC>(st, mat, d, K, idx, ldidx, val, ldval, lse);
+  else if (d.cols <= 256 * kHold) launch_row_top_as<256, VEC>(st, mat, d, K, idx, ldidx, val, ldval, lse);
+  else if (d.cols <= 512 * kHold) launch_row_top_as<512, VEC>(st, mat, d, K, idx, ldidx, val, ldval, lse);
+  else launch_row_top_as<1024, VEC>(st, mat, d, K, idx, ldidx, val, ldval, lse);
 }
 
 template <bool VEC, bool BOTH>
