@@ -22,16 +22,44 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 struct Frag {
   v8b hi, mid, lo;
 };
+// Two floats at a time: x - hi comes from the instruction that adds two bfloat16 products to a float, with the factors -1
+// and 0 (exact: the difference is a float); unpacking hi first would take two instructions more.  The factors are kept in
+// scalar registers: as literals the assembler takes -1 for the upper half only.
+struct Minus {
+  v2b first, second;
+};
+__device__ __forceinline__ Minus minus_ones() {
+  unsigned f = 0x0000bf80u, s = 0xbf800000u;
+  asm("" : "+s"(f), "+s"(s));
+  return {__builtin_bit_cast(v2b, f), __builtin_bit_cast(v2b, s)};
+}
+__device__ __forceinline__ void split2(float x, float y, v2b &hi, v2b &mid, v2b &lo) {
+  const Minus one = minus_ones();
+  hi = __builtin_convertvector((v2f){x, y}, v2b);
+  x = __builtin_amdgcn_fdot2_f32_bf16(hi, one.first, x, false);
+  y = __builtin_amdgcn_fdot2_f32_bf16(hi, one.second, y, false);
+  mid = __builtin_convertvector((v2f){x, y}, v2b);
+  x = __builtin_amdgcn_fdot2_f32_bf16(mid, one.first, x, false);
+  y = __builtin_amdgcn_fdot2_f32_bf16(mid, one.second, y, false);
+  lo = __builtin_convertvector((v2f){x, y}, v2b);
+}
+// the same with the parts unpacked and subtracted: where the matrix instructions keep the vector unit waiting anyway (the
+// tiled kernel), this measures 3 % faster than the above, in the kernels that split more than they multiply 6 % slower
+__device__ __forceinline__ void split2_apart(float x, float y, v2b &hi, v2b &mid, v2b &lo) {
+  hi = __builtin_convertvector((v2f){x, y}, v2b);
+  x -= (float)hi.x, y -= (float)hi.y;
+  mid = __builtin_convertvector((v2f){x, y}, v2b);
+  x -= (float)mid.x, y -= (float)mid.y;
+  lo = __builtin_convertvector((v2f){x, y}, v2b);
+}
+template <bool APART = false>
 __device__ __forceinline__ Frag split8(const float (&x)[8]) {
   Frag f;
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    const v2f v = {x[i], x[i + 1]};
-    const v2b h = __builtin_convertvector(v, v2b);
-    const v2f r = {v.x - (float)h.x, v.y - (float)h.y};
-    const v2b m = __builtin_convertvector(r, v2b);
-    const v2f q = {r.x - (float)m.x, r.y - (float)m.y};
-    const v2b l = __builtin_convertvector(q, v2b);
+    v2b h, m, l;
+    if (APART) split2_apart(x[i], x[i + 1], h, m, l);
+    else split2(x[i], x[i + 1], h, m, l);
     f.hi[i] = h.x, f.hi[i + 1] = h.y;
     f.mid[i] = m.x, f.mid[i + 1] = m.y;
     f.lo[i] = l.x, f.lo[i + 1] = l.y;
@@ -50,18 +78,21 @@ __device__ __forceinline__ v4f mfma6(const Frag &a, const Frag &b, v4f c) {
 }
 
 // ---- operand loads ------------------------------------------------------------------------------------------------
-// The 16x16x32 instruction: lane l holds A[l % 16][8 (l / 16) + e] and B[8 (l / 16) + e][l % 16], e = 0..7, and gets
-// D[4 (l / 16) + i][l % 16], i = 0..3.
+// The 16x16x32 instruction: lane l holds eight elements of row l % 16 of A and of column l % 16 of B, and gets
+// D[4 (l / 16) + i][l % 16], i = 0..3.  Which of a step's 32 inner indices the eight are is free as long as A and B agree:
+// with q = l / 16 they are 4 q .. 4 q + 3 and 16 + 4 q .. 16 + 4 q + 3, so that one load of 16 bytes per lane covers whole
+// 64-byte pieces of 16 rows.
+__device__ __forceinline__ int inner(int q, int e) { return 4 * q + (e & 3) + 4 * (e & 4); }
 
-// eight floats of one row, k .. k+7, zeros from K on
+// the lane's eight of a row at `row` (which points at the step's first), zeros from `left` on
 template <bool VEC>
-__device__ __forceinline__ void load_row8(const float *row, int k, int K, float (&x)[8]) {
-  if (VEC && k + 8 <= K) {
-    const v4f a = *reinterpret_cast<const v4f *>(row + k), b = *reinterpret_cast<const v4f *>(row + k + 4);
+__device__ __forceinline__ void load_row8(const float *row, int q, int left, float (&x)[8]) {
+  if (VEC && left >= 32) {
+    const v4f a = *reinterpret_cast<const v4f *>(row + 4 * q), b = *reinterpret_cast<const v4f *>(row + 16 + 4 * q);
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = k + e < K ? row[k + e] : 0.f;
+    for (int e = 0; e < 8; ++e) x[e] = inner(q, e) < left ? row[inner(q, e)] : 0.f;
   }
 }
 // NB neighbouring floats of a row from column c, zeros from C on
@@ -78,6 +109,23 @@ __device__ __forceinline__ void load_cols(const float *row, int c, int C, float 
     for (int j = 0; j < NB; ++j) x[j] = c + j < C ? row[c + j] : 0.f;
   }
 }
+
+// Rows whose lanes would each ask for another 16 bytes cost one request per lane; eight lanes that ask for 128 bytes of a
+// row cost one.  So a wave has the rows of a step copied into its own piece of LDS, eight rows per instruction, and
+// takes its operands from there.  Slot 8 r + c (16 bytes) holds the four floats c ^ (r & 7) of row r, so that the eight lanes
+// that read the same four of eight rows find them in different banks.
+__device__ __forceinline__ void stage_rows(const float *row, int lane, float *to) {  // `row`: of lane / 8, at the step's first
+  typedef __attribute__((address_space(1))) const void gvoid;
+  typedef __attribute__((address_space(3))) void lvoid;
+  __builtin_amdgcn_global_load_lds((gvoid *)(row + 4 * ((lane & 7) ^ (lane >> 3))), (lvoid *)to, 16, 0, 0);
+}
+__device__ __forceinline__ void staged_row8(const float *piece, int r, int q, float (&x)[8]) {
+  const v4f a = *reinterpret_cast<const v4f *>(piece + 32 * r + 4 * (q ^ (r & 7)));
+  const v4f b = *reinterpret_cast<const v4f *>(piece + 32 * r + 4 * ((4 + q) ^ (r & 7)));
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void staged_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void staged_taken() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // ---- which adapter ------------------------------------------------------------------------------------------------
 struct Stack {
@@ -176,8 +224,9 @@ template <int NB, int NW, bool VEC>
 __global__ __launch_bounds__(64 * NW) void narrow_kernel(const float *x, int ldx, int N, int K, const float *side, int lds,
                                                          Stack st, const int32_t *row_adapter, const int32_t *order,
                                                          int window, float *t, int ldt) {
+  __shared__ __align__(16) float stage_s[VEC ? NW * (16 + 16 * NB) * 32 : 4];
   __shared__ float part[NW][16][16 * NB + 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, q = lane >> 4;
   const int first_row = blockIdx.x * window, col0 = blockIdx.y * 16 * NB;
   const int row = lane < window ? row_of(order, first_row + lane, N) : -1;
   const int g = adapter_of(row_adapter, st.num, row);
@@ -199,11 +248,42 @@ __global__ __launch_bounds__(64 * NW) void narrow_kernel(const float *x, int ldx
     v4f acc[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[j] = (v4f){0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 32 * wave; k0 < K; k0 += 32 * NW) {
-      float a[8], b[NB][8];
-      load_row8<VEC>(xr, k0 + 8 * q, K, a);
+    int k0 = 32 * wave;
+    if (VEC && k0 + 32 <= K) {
+      float *piece = stage_s + wave * (16 + 16 * NB) * 32;
+      const float *sx[2], *sb[2 * NB];
 #pragma unroll
-      for (int j = 0; j < NB; ++j) load_row8<VEC>(br[j], k0 + 8 * q, K, b[j]);
+      for (int i = 0; i < 2; ++i) sx[i] = x + (size_t)max(__shfl(row, 8 * i + (lane >> 3), 64), 0) * ldx;
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) {
+        const int r = 8 * i + (lane >> 3);  // piece row 16 j + l: the stack's row NB l + j
+        sb[i] = side + (size_t)(lo + min(col0 + NB * (r & 15) + (r >> 4), rank - 1)) * lds;
+      }
+      auto ask = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) stage_rows(sx[i] + k, lane, piece + 256 * i);
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) stage_rows(sb[i] + k, lane, piece + 512 + 256 * i);
+      };
+      ask(k0);
+      for (; k0 + 32 <= K; k0 += 32 * NW) {
+        float a[8], b[NB][8];
+        staged_arrived();
+        staged_row8(piece, l15, q, a);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) staged_row8(piece + 512, 16 * j + l15, q, b[j]);
+        staged_taken();
+        if (k0 + 32 * NW + 32 <= K) ask(k0 + 32 * NW);
+        const Frag fa = split8(a);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[j] = mfma6(fa, split8(b[j]), acc[j]);
+      }
+    }
+    for (; k0 < K; k0 += 32 * NW) {
+      float a[8], b[NB][8];
+      load_row8<VEC>(xr + k0, q, K - k0, a);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) load_row8<VEC>(br[j] + k0, q, K - k0, b[j]);
       const Frag fa = split8(a);
 #pragma unroll
       for (int j = 0; j < NB; ++j) acc[j] = mfma6(fa, split8(b[j]), acc[j]);
@@ -255,13 +335,15 @@ struct WideArgs {
 // product with its rows of the stack is added to the run's rows only.
 template <int MB, int NB, int NW, bool NN, bool VEC>
 __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
-  constexpr int BM = 16 * MB, BN = 16 * NB;
-  __shared__ float part[NW][BM][BN];
+  constexpr int BM = 16 * MB, BN = 16 * NB, STAGED = NN ? BM : BM + BN;
+  constexpr int SHARED = VEC && STAGED * 32 > BM * BN ? STAGED * 32 : BM * BN;
+  __shared__ __align__(16) float stage_s[NW * SHARED];  // a wave's rows of a step; at the end its sums
+  float (*part)[BM][BN] = reinterpret_cast<float (*)[BM][BN]>(stage_s);
   // tiles of the same columns run on one of the 8 dies, so that a piece of W comes into one L2 only
   const int die = blockIdx.x & 7, local = blockIdx.x >> 3;
   const int tile_n = die + 8 * (local / p.tiles_m), tile_m = local % p.tiles_m;
   if (tile_n >= p.tiles_n) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, q = lane >> 4;
   const int m0 = tile_m * BM, n0 = tile_n * BN, c0 = n0 + NB * l15;
   const int row = lane < BM ? row_of(p.order, m0 + lane, p.N) : -1;
   int my_row[MB];
@@ -280,44 +362,107 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
   const float *wr[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) wr[j] = p.w + (size_t)min(c0 + j, p.C - 1) * p.ldw;
-  for (int k0 = 32 * wave; k0 < p.K; k0 += 32 * NW) {
+  struct Step {
     float a[MB][8], b[NB][8];
+  };
+  auto load = [&](int k0, int left, Step &s) {
 #pragma unroll
-    for (int m = 0; m < MB; ++m) load_row8<VEC>(xr[m], k0 + 8 * q, p.K, a[m]);
+    for (int m = 0; m < MB; ++m) load_row8<VEC>(xr[m] + k0, q, left, s.a[m]);
     if (NN) {
+      const float *w = p.w + (size_t)k0 * p.ldw;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int k = k0 + 8 * q + e;
         float v[NB] = {};
-        if (k < p.K) load_cols<NB, VEC>(p.w + (size_t)k * p.ldw, c0, p.C, v);
+        if (inner(q, e) < left) load_cols<NB, VEC>(w + (size_t)inner(q, e) * p.ldw, c0, p.C, v);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) b[j][e] = v[j];
+        for (int j = 0; j < NB; ++j) s.b[j][e] = v[j];
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < NB; ++j) load_row8<VEC>(wr[j], k0 + 8 * q, p.K, b[j]);
+      for (int j = 0; j < NB; ++j) load_row8<VEC>(wr[j] + k0, q, left, s.b[j]);
     }
+  };
+  auto multiply = [&](const Step &s) {
     Frag fa[MB];
 #pragma unroll
-    for (int m = 0; m < MB; ++m) fa[m] = split8(a[m]);
+    for (int m = 0; m < MB; ++m) fa[m] = split8(s.a[m]);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const Frag fb = split8(b[j]);
+      const Frag fb = split8(s.b[j]);
 #pragma unroll
       for (int m = 0; m < MB; ++m) acc[m][j] = mfma6(fa[m], fb, acc[m][j]);
     }
+  };
+  // the runs of equal adapters in the tile, and where the first that this wave takes has its rows of the stack: asked for
+  // now, used behind the product
+  Runs runs = {0, 0};
+  int first_lo = 0, first_rank = 0;
+  if (p.t) {
+    const int g = adapter_of(p.row_adapter, p.st.num, row);
+    runs = find_runs(g, lane);
+    unsigned long long left = runs.starts;
+    for (int i = 0; i < wave && left; ++i) left &= left - 1ull;
+    if (left) stack_rows(p.st, __shfl(g, __builtin_ctzll(left), 64), &first_lo, &first_rank);
+  }
+  constexpr int D = 32 * NW;
+  int k0 = 32 * wave;
+  if (VEC && k0 + 32 <= p.K) {
+    float *piece = stage_s + wave * STAGED * 32;
+    const float *sx[2 * MB], *sw[2 * NB];
+#pragma unroll
+    for (int i = 0; i < 2 * MB; ++i) sx[i] = p.x + (size_t)max(__shfl(row, 8 * i + (lane >> 3), 64), 0) * p.ldx;
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) {
+      const int r = 8 * i + (lane >> 3);  // piece row 16 j + l: row NB l + j of the tile's part of W
+      sw[i] = p.w + (size_t)min(n0 + NB * (r & 15) + (r >> 4), p.C - 1) * p.ldw;
+    }
+    float raw[8][NB];  // (NN: rows of W along the tile's columns, straight into registers)
+    auto ask = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < 2 * MB; ++i) stage_rows(sx[i] + k, lane, piece + 256 * i);
+      if (NN) {
+        const float *w = p.w + (size_t)k * p.ldw;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) load_cols<NB, VEC>(w + (size_t)inner(q, e) * p.ldw, c0, p.C, raw[e]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) stage_rows(sw[i] + k, lane, piece + 512 * MB + 256 * i);
+      }
+    };
+    ask(k0);
+    for (; k0 + 32 <= p.K; k0 += D) {
+      Step s;
+      staged_arrived();
+#pragma unroll
+      for (int m = 0; m < MB; ++m) staged_row8(piece, 16 * m + l15, q, s.a[m]);
+      if (NN) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int j = 0; j < NB; ++j) s.b[j][e] = raw[e][j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) staged_row8(piece + 512 * MB, 16 * j + l15, q, s.b[j]);
+      }
+      staged_taken();
+      if (k0 + D + 32 <= p.K) ask(k0 + D);
+      multiply(s);
+    }
+  }
+  for (; k0 < p.K; k0 += D) {
+    Step rest;
+    load(k0, p.K - k0, rest);
+    multiply(rest);
   }
 
   if (p.t) {
-    const int g = adapter_of(p.row_adapter, p.st.num, row);
-    const Runs runs = find_runs(g, lane);
     int turn = 0;
     for (unsigned long long left = runs.starts; left; left &= left - 1ull, ++turn) {
       if (turn % NW != wave) continue;
       const int s = __builtin_ctzll(left);
       const unsigned long long mask = run_mask(runs, s);
-      int lo, rank;
-      stack_rows(p.st, __shfl(g, s, 64), &lo, &rank);
+      int lo = first_lo, rank = first_rank;
+      if (turn >= NW) stack_rows(p.st, adapter_of(p.row_adapter, p.st.num, __shfl(row, s, 64)), &lo, &rank);
       v4f d[MB][NB];
 #pragma unroll
       for (int m = 0; m < MB; ++m)
@@ -327,7 +472,7 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
         float b[NB][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int k = k0 + 8 * q + e;
+          const int k = k0 + inner(q, e);
           float v[NB] = {};
           if (k < rank) load_cols<NB, VEC>(p.side + (size_t)(lo + k) * p.ldside, c0, p.C, v);
 #pragma unroll
@@ -337,7 +482,7 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
 #pragma unroll
         for (int m = 0; m < MB; ++m) {
           float a[8];
-          load_row8<VEC>(p.t + (size_t)max(my_row[m], 0) * p.ldt, k0 + 8 * q, rank, a);
+          load_row8<VEC>(p.t + (size_t)max(my_row[m], 0) * p.ldt + k0, q, rank - k0, a);
           fa[m] = split8(a);
         }
 #pragma unroll
@@ -357,6 +502,7 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
     }
   }
 
+  __syncthreads();  // (the pieces of LDS have been read: now they take the sums)
 #pragma unroll
   for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -400,12 +546,8 @@ __device__ __forceinline__ v16f mfma6_32(const Frag &a, const Frag &b, v16f c) {
 __device__ __forceinline__ void split4(v4f x, v4b &hi, v4b &mid, v4b &lo) {
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
-    const v2f v = {x[i], x[i + 1]};
-    const v2b h = __builtin_convertvector(v, v2b);
-    const v2f r = {v.x - (float)h.x, v.y - (float)h.y};
-    const v2b m = __builtin_convertvector(r, v2b);
-    const v2f q = {r.x - (float)m.x, r.y - (float)m.y};
-    const v2b l = __builtin_convertvector(q, v2b);
+    v2b h, m, l;
+    split2_apart(x[i], x[i + 1], h, m, l);
     hi[i] = h.x, hi[i + 1] = h.y;
     mid[i] = m.x, mid[i + 1] = m.y;
     lo[i] = l.x, lo[i + 1] = l.y;
@@ -438,7 +580,7 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
   const int group = id / (4 * p.tiles_n), in_group = min(4, p.tiles_m - 4 * group), rest = id - group * 4 * p.tiles_n;
   const int m0 = (4 * group + rest % in_group) * BM, n0 = (rest / in_group) * BN;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, l31 = lane & 31, half = lane >> 5;
 
   const float *ar[AU];
@@ -510,7 +652,7 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
     for (int u = 0; u < BC; ++u) {
       const int n = (tid + 512 * u) % BN, c = (tid + 512 * u) / BN;
       if (c < 4) {
-        const Frag f = split8(rc[u]);
+        const Frag f = split8<true>(rc[u]);
         const int s = A_SLOTS + slot_of(n, c);
         lds[buf][0][s] = f.hi, lds[buf][1][s] = f.mid, lds[buf][2][s] = f.lo;
       }
@@ -594,7 +736,8 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
           for (int i = 0; i < 16; ++i) d[n][i] = 0.f;
         for (int k0 = 0; k0 < rank; k0 += 16) {
           float a[8];
-          load_row8<VEC>(tr, k0 + 8 * half, rank, a);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a[e] = k0 + 8 * half + e < rank ? tr[k0 + 8 * half + e] : 0.f;
           const Frag fa = split8(a);
 #pragma unroll
           for (int n = 0; n < NB; ++n) {
@@ -645,51 +788,97 @@ struct GradArgs {
   const float *wide; int ldwide; int C;
   float *grad; int ldgrad;
 };
-template <int NB, int NW, bool VEC>
+template <int MB, int NB, int NW, bool VEC>
 __global__ __launch_bounds__(64 * NW) void grad_kernel(GradArgs down, GradArgs up, int N, Stack st, const int32_t *order,
                                                        const int32_t *row_begin, int col_tiles, int rank_blocks) {
-  __shared__ float part[NW][16][16 * NB];
+  __shared__ float part[NW > 1 ? NW : 1][16 * MB][16 * NB];
   const bool is_up = blockIdx.y >= (unsigned)rank_blocks;
   const GradArgs &p = is_up ? up : down;
-  const int k_base = (blockIdx.y - (is_up ? rank_blocks : 0)) * 16;
+  const int k_base = (blockIdx.y - (is_up ? rank_blocks : 0)) * 16 * MB;
   const int g = blockIdx.x / col_tiles, n0 = (blockIdx.x % col_tiles) * 16 * NB;
   if (n0 >= p.C) return;
   int lo, rank;
   stack_rows(st, g, &lo, &rank);
   if (k_base >= rank) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, q = lane >> 4;
   const int begin = min(max(row_begin[g], 0), N), end = min(row_begin[g + 1], N), c0 = n0 + NB * l15;
-  v4f acc[NB];
+  v4f acc[MB][NB];
 #pragma unroll
-  for (int j = 0; j < NB; ++j) acc[j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[m][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  int mine = begin + 32 * wave + lane < end && lane < 32 ? row_of(order, begin + 32 * wave + lane, N) : -1;
   for (int r0 = begin + 32 * wave; r0 < end; r0 += 32 * NW) {
-    const int mine = lane < 32 && r0 + lane < end ? row_of(order, r0 + lane, N) : -1;
-    float a[8], b[NB][8];
+    float a[MB][8], b[NB][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int r = __shfl(mine, 8 * q + e, 64);
-      a[e] = r >= 0 && k_base + l15 < rank ? p.narrow[(size_t)r * p.ldnarrow + k_base + l15] : 0.f;
+      const int r = __shfl(mine, inner(q, e), 64);
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+        a[m][e] = r >= 0 && k_base + 16 * m + l15 < rank ? p.narrow[(size_t)r * p.ldnarrow + k_base + 16 * m + l15] : 0.f;
       float v[NB] = {};
       if (r >= 0) load_cols<NB, VEC>(p.wide + (size_t)r * p.ldwide, c0, p.C, v);
 #pragma unroll
       for (int j = 0; j < NB; ++j) b[j][e] = v[j];
     }
-    const Frag fa = split8(a);
+    const int later = r0 + 32 * NW + lane;
+    mine = later < end && lane < 32 ? row_of(order, later, N) : -1;
+    Frag fa[MB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[j] = mfma6(fa, split8(b[j]), acc[j]);
+    for (int m = 0; m < MB; ++m) fa[m] = split8(a[m]);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const Frag fb = split8(b[j]);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) acc[m][j] = mfma6(fa[m], fb, acc[m][j]);
+    }
+  }
+  if (NW == 1) {  // nothing to add up
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const int k = k_base + 16 * m + 4 * q + i;
+          if (k < rank && c0 + j < p.C) p.grad[(size_t)(lo + k) * p.ldgrad + c0 + j] = acc[m][j][i];
+        }
+    return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int m = 0; m < MB; ++m)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) part[wave][4 * q + i][NB * l15 + j] = acc[j][i];
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) part[wave][16 * m + 4 * q + i][NB * l15 + j] = acc[m][j][i];
   __syncthreads();
-  for (int e = threadIdx.x; e < 256 * NB; e += 64 * NW) {
+  for (int e = threadIdx.x; e < 256 * MB * NB; e += 64 * NW) {
     const int k = e / (16 * NB), c = e % (16 * NB);
     if (k_base + k >= rank || n0 + c >= p.C) continue;
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) v += part[w][k][c];
     p.grad[(size_t)(lo + k_base + k) * p.ldgrad + n0 + c] = v;
+  }
+}
+template <int MB, int NW, bool VEC>
+void launch_grad(hipStream_t st, const GradArgs &down, const GradArgs &up, int N, const Stack &stack, const int32_t *order,
+                 const int32_t *row_begin, int col_tiles) {
+  const int rank_blocks = (stack.max_rank + 16 * MB - 1) / (16 * MB);
+  const dim3 grid((unsigned)col_tiles * stack.num, 2 * rank_blocks);
+  grad_kernel<MB, 2, NW, VEC><<<grid, 64 * NW, 0, st>>>(down, up, N, stack, order, row_begin, col_tiles, rank_blocks);
+}
+template <bool VEC>
+void launch_grads(hipStream_t st, const GradArgs &down, const GradArgs &up, int N, const Stack &stack, const int32_t *order,
+                  const int32_t *row_begin, int col_tiles) {
+  // one wave for adapters of few rows
+  const bool few = N <= 64 * (long long)stack.num;
+  if (stack.max_rank <= 16) {
+    if (few) launch_grad<1, 1, VEC>(st, down, up, N, stack, order, row_begin, col_tiles);
+    else launch_grad<1, 8, VEC>(st, down, up, N, stack, order, row_begin, col_tiles);
+  } else {
+    if (few) launch_grad<2, 1, VEC>(st, down, up, N, stack, order, row_begin, col_tiles);
+    else launch_grad<2, 8, VEC>(st, down, up, N, stack, order, row_begin, col_tiles);
   }
 }
 
@@ -715,12 +904,12 @@ void launch_narrow(hipStream_t st, const float *x, int ldx, int N, int K, const 
     narrow_kernel<2, 8, VEC><<<grid, 512, 0, st>>>(x, ldx, N, K, side, ldside, stack, row_adapter, order, window, t, ldt);
 }
 
-template <int MB, int NB, bool NN, bool VEC>
+template <int MB, int NB, int NW, bool NN, bool VEC>
 void launch_wide_tile(hipStream_t st, WideArgs p) {
   p.tiles_m = (p.N + 16 * MB - 1) / (16 * MB);
   p.tiles_n = (p.C + 16 * NB - 1) / (16 * NB);
   const unsigned blocks = 8u * ((p.tiles_n + 7) / 8) * (unsigned)p.tiles_m;
-  wide_kernel<MB, NB, 8, NN, VEC><<<blocks, 512, 0, st>>>(p);
+  wide_kernel<MB, NB, NW, NN, VEC><<<blocks, 64 * NW, 0, st>>>(p);
 }
 template <int WM, int WN, int MB, int NB, bool NN, bool VEC>
 void launch_tiled(hipStream_t st, WideArgs p) {
@@ -729,13 +918,29 @@ void launch_tiled(hipStream_t st, WideArgs p) {
   const unsigned blocks = 8u * (((unsigned)p.tiles_m * p.tiles_n + 7) / 8);
   tiled_kernel<WM, WN, MB, NB, NN, VEC><<<blocks, 512, 0, st>>>(p);
 }
+// Which kernel and tile.  The tiles of a product are worked off in rounds of one per compute unit; what a round takes was
+// measured with 2048 inner indices (us): 16 rows x 16 columns 7, 16 x 32 8, 32 x 64 18, 64 x 128 66, 128 x 128 95, 256 x 128
+// 170.  E.g. 2048 columns: 1 row 16x16 7 us (16x32 7.5, 32x64 16); 64 rows 16x32 8 (16x16 10, 32x64 17); 256 rows 32x64 18 (16x32
+// 31, 64x128 64); 1024 rows 64x128 68 (32x64 74, 128x128 93); 2048 rows 128x128 106 (64x128 113, 256x128 156); 4096 rows
+// 256x128 176 (128x128 197).
 template <bool NN, bool VEC>
 void launch_wide(hipStream_t st, const WideArgs &p) {
-  if (p.N >= 1024) return launch_tiled<4, 2, 2, 2, NN, VEC>(st, p);
-  const long long rows16 = (p.N + 15) / 16, cols16 = (p.C + 15) / 16;
-  if (rows16 * cols16 <= 256) launch_wide_tile<1, 1, NN, VEC>(st, p);
-  else if (rows16 * cols16 <= 1024) launch_wide_tile<1, 2, NN, VEC>(st, p);
-  else launch_wide_tile<2, 4, NN, VEC>(st, p);
+  static const struct { int rows, cols, round; } kTiles[] = {{16, 16, 7}, {16, 32, 8}, {32, 64, 18}, {64, 128, 66}, {128, 128, 95}, {256, 128, 170}};
+  int best = 0;
+  long long least = 0;
+  for (int i = 0; i < 6; ++i) {
+    const long long tiles = (long long)((p.N + kTiles[i].rows - 1) / kTiles[i].rows) * ((p.C + kTiles[i].cols - 1) / kTiles[i].cols);
+    const long long cost = (tiles + 255) / 256 * kTiles[i].round;
+    if (i == 0 || cost < least) best = i, least = cost;
+  }
+  switch (best) {
+    case 0: return launch_wide_tile<1, 1, 8, NN, VEC>(st, p);
+    case 1: return launch_wide_tile<1, 2, 16, NN, VEC>(st, p);
+    case 2: return launch_wide_tile<2, 4, 8, NN, VEC>(st, p);
+    case 3: return launch_tiled<2, 4, 1, 1, NN, VEC>(st, p);
+    case 4: return launch_tiled<4, 2, 1, 2, NN, VEC>(st, p);
+    default: return launch_tiled<4, 2, 2, 2, NN, VEC>(st, p);
+  }
 }
 
 int check_adapters(const khAdapters *ad, const int32_t *row_adapter, int32_t N, int32_t I, int32_t O) {
@@ -849,19 +1054,17 @@ KH_EXPORT int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t 
     if (rc != KH_OK) return rc;
   }
   if (!grads || ad->rows == 0) return KH_OK;
-  const int rank_blocks = (ad->max_rank + 15) / 16;
   GradArgs gd = {u, ldu, in, ldin, gdown != nullptr ? I : 0, gdown, ldgdown};
   GradArgs gu = {t, ldt, e, lde, gup != nullptr ? O : 0, gup, ldgup};
   const int cols = std::max(gd.C, gu.C);
   if (cols == 0) return KH_OK;
-  const int col_tiles = (cols + 63) / 64;
+  const int col_tiles = (cols + 31) / 32;
   if ((long long)col_tiles * ad->num > 0x7fffffffLL) {
     snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "gradients of %d adapters of %d columns: too many", ad->num, cols);
     return KH_ERR_TOO_LARGE;
   }
-  const dim3 grid((unsigned)col_tiles * ad->num, 2 * rank_blocks);
   const bool vec = (gdown == nullptr || vec_ok(in, ldin)) && (gup == nullptr || vec_ok(e, lde));
-  if (vec) grad_kernel<4, 8, true><<<grid, 512, 0, st>>>(gd, gu, N, stack, order, row_begin, col_tiles, rank_blocks);
-  else grad_kernel<4, 8, false><<<grid, 512, 0, st>>>(gd, gu, N, stack, order, row_begin, col_tiles, rank_blocks);
+  if (vec) launch_grads<true>(st, gd, gu, N, stack, order, row_begin, col_tiles);
+  else launch_grads<false>(st, gd, gu, N, stack, order, row_begin, col_tiles);
   return kh::launch_status();
 }
