@@ -226,6 +226,8 @@ __global__ __launch_bounds__(64 * NW) void narrow_kernel(const float *x, int ldx
                                                          int window, float *t, int ldt) {
   __shared__ __align__(16) float stage_s[VEC ? NW * (16 + 16 * NB) * 32 : 4];
   __shared__ float part[NW][16][16 * NB + 4];
+  __shared__ int rows_s[16];
+  __shared__ float scale_s[16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, q = lane >> 4;
   const int first_row = blockIdx.x * window, col0 = blockIdx.y * 16 * NB;
   const int row = lane < window ? row_of(order, first_row + lane, N) : -1;
@@ -233,6 +235,10 @@ __global__ __launch_bounds__(64 * NW) void narrow_kernel(const float *x, int ldx
   const Runs runs = find_runs(g, lane);
   const int my_row = __shfl(row, l15, 64);
   const float *xr = x + (size_t)max(my_row, 0) * ldx;
+  if (wave == 0 && lane < 16) {  // for the end; asked for now
+    rows_s[lane] = row;
+    scale_s[lane] = g >= 0 && st.scale ? st.scale[g] : 1.f;
+  }
   v4f total[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) total[j] = (v4f){0.f, 0.f, 0.f, 0.f};
@@ -301,13 +307,12 @@ __global__ __launch_bounds__(64 * NW) void narrow_kernel(const float *x, int ldx
   __syncthreads();
   for (int e = threadIdx.x; e < window * 16 * NB; e += 64 * NW) {
     const int m = e / (16 * NB), c = e % (16 * NB);
-    const int r = row_of(order, first_row + m, N);
+    const int r = rows_s[m];
     if (r < 0 || col0 + c >= st.max_rank) continue;
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) v += part[w][m][c];
-    const int ga = adapter_of(row_adapter, st.num, r);
-    if (ga >= 0 && st.scale) v *= st.scale[ga];
+    v *= scale_s[m];
     t[(size_t)r * ldt + col0 + c] = v;
   }
 }
@@ -339,6 +344,8 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
   constexpr int SHARED = VEC && STAGED * 32 > BM * BN ? STAGED * 32 : BM * BN;
   __shared__ __align__(16) float stage_s[NW * SHARED];  // a wave's rows of a step; at the end its sums
   float (*part)[BM][BN] = reinterpret_cast<float (*)[BM][BN]>(stage_s);
+  __shared__ int rows_s[BM];
+  static_assert(64 * NW % BN == 0, "a thread finishes one column");
   // tiles of the same columns run on one of the 8 dies, so that a piece of W comes into one L2 only
   const int die = blockIdx.x & 7, local = blockIdx.x >> 3;
   const int tile_n = die + 8 * (local / p.tiles_m), tile_m = local % p.tiles_m;
@@ -393,6 +400,9 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
       for (int m = 0; m < MB; ++m) acc[m][j] = mfma6(fa[m], fb, acc[m][j]);
     }
   };
+  if (wave == 0 && lane < BM) rows_s[lane] = row;
+  const int my_c = n0 + threadIdx.x % BN;
+  const float my_bias = p.bias && my_c < p.C ? p.bias[my_c] : 0.f;  // for the end; asked for now
   // the runs of equal adapters in the tile, and where the first that this wave takes has its rows of the stack: asked for
   // now, used behind the product
   Runs runs = {0, 0};
@@ -503,6 +513,15 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
   }
 
   __syncthreads();  // (the pieces of LDS have been read: now they take the sums)
+  constexpr int EACH = BM * BN / (64 * NW) > 0 ? BM * BN / (64 * NW) : 1;
+  float y[EACH];
+  if (p.y) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int m = (threadIdx.x + 64 * NW * i) / BN, r = m < BM ? rows_s[m] : -1;
+      y[i] = r >= 0 && my_c < p.C ? p.y[(size_t)r * p.ldy + my_c] : 0.f;
+    }
+  }
 #pragma unroll
   for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -510,21 +529,17 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) part[wave][16 * m + 4 * q + i][NB * l15 + j] = acc[m][j][i];
   __syncthreads();
-  for (int e = threadIdx.x; e < BM * BN; e += 64 * NW) {
-    const int m = e / BN, c = n0 + e % BN;
-    const int r = row_of(p.order, m0 + m, p.N);
-    if (r < 0 || c >= p.C) continue;
-    float v = p.bias ? p.bias[c] : 0.f;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int m = (threadIdx.x + 64 * NW * i) / BN, r = m < BM ? rows_s[m] : -1;
+    if (r < 0 || my_c >= p.C) continue;
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) sum += part[w][m][e % BN];
-    v += sum;
+    for (int w = 0; w < NW; ++w) sum += part[w][m][threadIdx.x % BN];
+    float v = my_bias + sum;
     if (p.act == KH_ACT_SIGMOID) v = kh::sigmoidf(v);
-    if (p.y) {
-      const float yv = p.y[(size_t)r * p.ldy + c];
-      v = v * yv * (1.f - yv);
-    }
-    p.out[(size_t)r * p.ldout + c] = v;
+    if (p.y) v = v * y[i] * (1.f - y[i]);
+    p.out[(size_t)r * p.ldout + my_c] = v;
   }
 }
 
