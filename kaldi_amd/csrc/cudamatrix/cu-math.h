@@ -82,6 +82,18 @@ void FindRowMaxId(const CuMatrix<Real> &mat, CuStlVector<int32> *id) {
   id->Resize(mat.NumRows());
   CU_SAFE_CALL(hipF_find_row_max_id(detail::S(), mat.Data(), NULL, id->Data(), mat.Dim()));
 }
+/// The k largest elements of every row in descending order, equal ones by column: id[r * k + i] is the column of val(r, i),
+/// -1 behind the row's end; lse (may be NULL): log(sum(exp(row))).  No counterpart in the reference.
+template <typename Real>
+void RowTop(const CuMatrix<Real> &mat, int32 k, CuStlVector<int32> *id, CuMatrix<Real> *val, CuVector<Real> *lse) {
+  CuProfileScope p(__func__);
+  KALDI_ASSERT(k >= 1);
+  id->Resize(static_cast<size_t>(mat.NumRows()) * k);
+  val->Resize(mat.NumRows(), k);
+  if (lse) lse->Resize(mat.NumRows());
+  CU_SAFE_CALL(hipF_row_top(detail::S(), mat.Data(), mat.Dim(), k, id->Data(), k, val->Data(), val->Stride() ? val->Stride() : k,
+                            lse ? lse->Data() : NULL));
+}
 /// log_post_tgt[r] = log(out[r,tgt[r]]); out[r,tgt[r]] -= 1
 template <typename Real>
 void DiffXent(const CuStlVector<int32> &tgt, CuMatrix<Real> *net_out_or_diff, CuVector<Real> *log_post_tgt) {

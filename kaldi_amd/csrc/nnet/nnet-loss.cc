@@ -121,6 +121,38 @@ BaseFloat Xent::GetFrameAccuracy() {
   return 100.0 * correct_ / frames_;
 }
 
+void Distill::Eval(const CuMatrix<BaseFloat> &net_out, const CuStlVector<int32> &id, const CuMatrix<BaseFloat> &val,
+                   const CuStlVector<int32> *label, const CuVector<BaseFloat> *weight, CuMatrix<BaseFloat> *diff) {
+  CuProfileScope p("Distill::Eval");
+  const int32 n = net_out.NumRows(), k = val.NumCols();
+  KALDI_ASSERT(val.NumRows() == n && id.Dim() == static_cast<size_t>(n) * k);
+  KALDI_ASSERT(label == NULL || static_cast<int32>(label->Dim()) == n);
+  KALDI_ASSERT(weight == NULL || static_cast<int32>(weight->Dim()) == n);
+  if (n == 0) return;
+  if (diff && diff != &net_out) diff->Resize(n, net_out.NumCols());
+  row_loss_.Resize(n);
+  CU_SAFE_CALL(hipF_distill_eval(S(), net_out.Data(), net_out.Dim(), id.Data(), k, val.Data(), val.Stride(), k,
+                                 label ? label->Data() : NULL, weight ? weight->Data() : NULL, temperature_, hard_weight_,
+                                 diff ? diff->Data() : NULL, diff ? diff->Stride() : 0, row_loss_.Data(), stats_.Loss()));
+  frames_ += n;
+}
+
+void Distill::GetStats(int64 *frames, double *loss) {
+  double l = 0.0;
+  stats_.Fetch(NULL, NULL, &l);
+  stats_.Reset();
+  loss_ += l;
+  if (frames) *frames = frames_;
+  if (loss) *loss = loss_;
+}
+
+std::string Distill::Report() {
+  GetStats(NULL, NULL);
+  std::ostringstream oss;
+  oss << "Distill:" << loss_ << " frames:" << frames_ << " err/frm:" << loss_ / frames_;
+  return oss.str();
+}
+
 void Mse::Eval(const CuMatrix<BaseFloat> &net_out, const CuMatrix<BaseFloat> &target, CuMatrix<BaseFloat> *diff) {
   CuProfileScope p("Mse::Eval");
   KALDI_ASSERT(net_out.NumCols() == target.NumCols());

@@ -78,6 +78,32 @@ std::string Report();
   CuVector<BaseFloat> log_post_tgt_;
 };
 
+/// Cross entropy towards a teacher's largest logits (cu::RowTop of its outputs before the softmax) at a temperature, mixed
+/// with hard labels: hipF_distill_eval has the formulas.  No counterpart in the reference, whose Xent::Eval knows whole
+/// target matrices.  Takes the network's outputs BEFORE the softmax; diff is the derivative with respect to them.
+class Distill {
+ public:
+  explicit Distill(BaseFloat temperature = 1.0, BaseFloat hard_weight = 0.0)
+      : temperature_(temperature), hard_weight_(hard_weight), frames_(0), loss_(0.0) {}
+  ~Distill() {}
+  /// id / val: k = val.NumCols() entries per row as cu::RowTop leaves them (id dense); label: one per row, needed when the
+  /// hard weight is not 0; weight: one per row or NULL.  diff may be NULL (the loss alone) or &net_out.
+  void Eval(const CuMatrix<BaseFloat> &net_out, const CuStlVector<int32> &id, const CuMatrix<BaseFloat> &val,
+            const CuStlVector<int32> *label, const CuVector<BaseFloat> *weight, CuMatrix<BaseFloat> *diff);
+  /// losses of the rows of the last Eval (device)
+  const CuVector<BaseFloat> &RowLoss() const { return row_loss_; }
+  std::string Report();
+  /// totals so far (blocking)
+  void GetStats(int64 *frames, double *loss);
+
+ private:
+  BaseFloat temperature_, hard_weight_;
+  int64 frames_;
+  double loss_;
+  DeviceStats stats_;
+  CuVector<BaseFloat> row_loss_;
+};
+
 class Mse {
  public:
   Mse() : frames_(0), loss_(0.0) {}
