@@ -495,7 +495,8 @@ int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int
  * together into tiles: give hipI32_adapter_plan's where neighbouring rows have different adapters, NULL where they lie
  * together already (utterances, single frames).  The result does not depend on it beyond rounding.  `t` is what
  * the backward pass needs; bias may be NULL.  out and t must not overlap an input.  Rows behind N and columns
- * behind O (max_rank) are left as they are.  Uses no library workspace: may be captured into a graph.
+ * behind O (max_rank) are left as they are.  Uses no library workspace: may be captured into a graph.  A row of t has
+ * the same bits whoever shares its call, and with hipK_gemm_row_invariant(1) so has a row of out.
  * Arithmetic: every float is taken as the sum of three bfloat16 numbers (24 bits of mantissa: exact) and a product
  * of two floats as the six largest of the nine part products, on the matrix cores with float sums; what is left out
  * is below 2^-26 of the product, less than one rounding of a float product.  An infinity or NaN in a row of `in`

@@ -950,12 +950,14 @@ void launch_tiled(hipStream_t st, WideArgs p) {
 template <bool NN, bool VEC>
 void launch_wide(hipStream_t st, const WideArgs &p) {
   static const struct { int rows, cols, round; } kTiles[] = {{16, 16, 7}, {16, 32, 8}, {32, 64, 18}, {64, 128, 66}, {128, 128, 95}, {256, 128, 170}};
-  int best = 0;
+  // (hipK_gemm_row_invariant: the tiled kernels only, which sum an element in the same order whatever their tile)
+  const int first = kh::gemm_row_invariant() ? 3 : 0;
+  int best = first;
   long long least = 0;
-  for (int i = 0; i < 6; ++i) {
+  for (int i = first; i < 6; ++i) {
     const long long tiles = (long long)((p.N + kTiles[i].rows - 1) / kTiles[i].rows) * ((p.C + kTiles[i].cols - 1) / kTiles[i].cols);
     const long long cost = (tiles + 255) / 256 * kTiles[i].round;
-    if (i == 0 || cost < least) best = i, least = cost;
+    if (i == first || cost < least) best = i, least = cost;
   }
   switch (best) {
     case 0: return launch_wide_tile<1, 1, 8, NN, VEC>(st, p);

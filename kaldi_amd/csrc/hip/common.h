@@ -44,6 +44,9 @@ int static_scratch_setup(int device);
 // The arrival counter of stream `st` (device memory, zero whenever no kernel that uses it is queued).
 int stream_ticket(hipStream_t st, unsigned **ticket);
 
+// Whether hipK_gemm_row_invariant is on.
+bool gemm_row_invariant();
+
 // What the row-softmax finish of a GEMM needs to go on to Xent::EvalVec in the same kernel.
 struct XentArgs {
   const int32_t *tgt;

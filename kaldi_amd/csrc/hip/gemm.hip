@@ -572,6 +572,9 @@ KH_EXPORT int hipK_gemm_force_plan(int bm, int bn, int splitk) {
   return KH_OK;
 }
 
+namespace kh {
+bool gemm_row_invariant() { return row_invariant; }
+}
 KH_EXPORT int hipK_gemm_row_invariant(int on) {
   row_invariant = on != 0;
   return KH_OK;
