@@ -148,7 +148,7 @@ constexpr int kCap = 1024;  // candidates of a chunk, next to the KH_MAX_TOP of 
 // elements that reach the bound are collected in LDS and ranked by counting; the K largest are kept.  Where more than kCap reach the bound (large values crowded into few groups, many equal ones), and
 // where the chunk holds a NaN or +inf, a bound on the distinct keys is found by bisection over the chunk.
 template <int THREADS, bool VEC, bool AHEAD>
-__global__ __launch_bounds__(THREADS, AHEAD ? 4 : 8) void row_top_kernel(const float *mat, MatrixDim d, int K, int32_t *idx, int ldidx,
+__global__ __launch_bounds__(THREADS, AHEAD ? 4 : THREADS == 64 ? 3 : 8) void row_top_kernel(const float *mat, MatrixDim d, int K, int32_t *idx, int ldidx,
                                                           float *val, int ldval, float *lse) {
   constexpr int G = THREADS < 256 ? THREADS : 256, per = THREADS / G, waves = THREADS / 64, chunk = THREADS * kHold;
   __shared__ __align__(16) float ahead[AHEAD ? chunk : 4];
@@ -575,7 +575,7 @@ void launch_row_top_as(hipStream_t st, const float *mat, MatrixDim d, int K, int
   // as many workgroups as run at once, each with its share of the rows
   constexpr unsigned by_lds = 163840u / (THREADS * kHold * 4u + (kCap + 2 * KH_MAX_TOP) * 8u + 2048u);
   const unsigned rows = (unsigned)d.rows, most = 256u * by_lds;
-  if (AHEAD) row_top_kernel<THREADS, VEC, true><<<rows < most ? rows : most, THREADS, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
+  if constexpr (AHEAD) row_top_kernel<THREADS, VEC, true><<<rows < most ? rows : most, THREADS, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
   else row_top_kernel<THREADS, VEC, false><<<rows, THREADS, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
 }
 template <bool VEC>

@@ -283,6 +283,7 @@ def test_no_adapters_no_rows_no_inputs(hip):
     ad = c.adapters()
     one = h.DevMatrix(4, 8)
     h.call("hipF_adapter_forward", None, 0, 0, 6, 5, None, 5, one.ptr, 8, None, ctypes.byref(ad), one.ptr, None, None, 3, None, 6)
+    h.call("hipF_adapter_forward", None, 0, 0, 6, 5, None, 0, one.ptr, 8, None, ctypes.byref(ad), one.ptr, None, None, 0, None, 0)
     # no inputs: the bias alone
     out = h.DevMatrix(4, 6)
     t = h.DevMatrix.from_numpy(np.full((4, 3), 7, f32))
