@@ -493,7 +493,8 @@ int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int
  *   out(N x O)       out[r,:] = act( bias + in[r,:] * W^T + t[r,:] * up_g )
  * with g = row_adapter[r].  `order` (may be NULL: the rows as they stand) is the sequence in which rows are put
  * together into tiles: give hipI32_adapter_plan's where neighbouring rows have different adapters, NULL where they lie
- * together already (utterances, single frames).  The result does not depend on it beyond rounding.  `t` is what
+ * together already (utterances, single frames).  The result does not depend on it beyond rounding (a row that a broken
+ * order does not list may stay unwritten).  `t` is what
  * the backward pass needs; bias may be NULL.  out and t must not overlap an input.  Rows behind N and columns
  * behind O (max_rank) are left as they are.  Uses no library workspace: may be captured into a graph.  A row of t has
  * the same bits whoever shares its call, and with hipK_gemm_row_invariant(1) so has a row of out.

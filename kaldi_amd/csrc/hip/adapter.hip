@@ -221,24 +221,37 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int32_t *row_adapter, 
 // inner dimension in turn and add up through LDS in a fixed order.  A window of several adapters is gone through
 // once per run of equal adapters; only the run's rows are kept from a pass, so nothing of one row reaches another.  Bound
 // by reading x (4096 x 2048: 16 us, 2.1 TB/s) or, for few rows, by latency (1 to 64 rows: 6.3 us, with 4, 8 or 16 waves).
+struct NarrowArgs {
+  const float *x; int ldx, N, K;
+  const float *side; int ldside;
+  Stack st;
+  const int32_t *row_adapter, *order;
+  int window;
+  float *t; int ldt;
+};
 template <int NB, int NW, bool VEC>
-__global__ __launch_bounds__(64 * NW) void narrow_kernel(const float *x, int ldx, int N, int K, const float *side, int lds,
-                                                         Stack st, const int32_t *row_adapter, const int32_t *order,
-                                                         int window, float *t, int ldt) {
-  __shared__ __align__(16) float stage_s[VEC ? NW * (16 + 16 * NB) * 32 : 4];
-  __shared__ float part[NW][16][16 * NB + 4];
-  __shared__ int rows_s[16];
-  __shared__ float scale_s[16];
+struct NarrowShared {
+  float stage[VEC ? NW * (16 + 16 * NB) * 32 : 4];
+  float part[NW][16][16 * NB + 4];
+  int rows[16];
+  float scale[16];
+};
+template <int NB, int NW, bool VEC>
+__device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, int block_y, NarrowShared<NB, NW, VEC> &sh) {
+  const float *x = p.x, *side = p.side;
+  const int ldx = p.ldx, N = p.N, K = p.K, lds = p.ldside, window = p.window;
+  const Stack &st = p.st;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, q = lane >> 4;
-  const int first_row = blockIdx.x * window, col0 = blockIdx.y * 16 * NB;
+  const int first_row = block_x * window, col0 = block_y * 16 * NB;
+  const int32_t *order = window > 1 ? p.order : nullptr;  // (nothing to put together: a load less to wait for, 1.4 us)
   const int row = lane < window ? row_of(order, first_row + lane, N) : -1;
-  const int g = adapter_of(row_adapter, st.num, row);
+  const int g = adapter_of(p.row_adapter, st.num, row);
   const Runs runs = find_runs(g, lane);
   const int my_row = __shfl(row, l15, 64);
   const float *xr = x + (size_t)max(my_row, 0) * ldx;
   if (wave == 0 && lane < 16) {  // for the end; asked for now
-    rows_s[lane] = row;
-    scale_s[lane] = g >= 0 && st.scale ? st.scale[g] : 1.f;
+    sh.rows[lane] = row;
+    sh.scale[lane] = g >= 0 && st.scale ? st.scale[g] : 1.f;
   }
   v4f total[NB];
 #pragma unroll
@@ -257,7 +270,7 @@ __global__ __launch_bounds__(64 * NW) void narrow_kernel(const float *x, int ldx
     for (int j = 0; j < NB; ++j) acc[j] = (v4f){0.f, 0.f, 0.f, 0.f};
     int k0 = 32 * wave;
     if (VEC && k0 + 32 <= K) {
-      float *piece = stage_s + wave * (16 + 16 * NB) * 32;
+      float *piece = sh.stage + wave * (16 + 16 * NB) * 32;
       const float *sx[2], *sb[2 * NB];
 #pragma unroll
       for (int i = 0; i < 2; ++i) sx[i] = x + (size_t)max(__shfl(row, 8 * i + (lane >> 3), 64), 0) * ldx;
@@ -304,21 +317,27 @@ __global__ __launch_bounds__(64 * NW) void narrow_kernel(const float *x, int ldx
 #pragma unroll
   for (int j = 0; j < NB; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[wave][4 * q + i][NB * l15 + j] = total[j][i];
+    for (int i = 0; i < 4; ++i) sh.part[wave][4 * q + i][NB * l15 + j] = total[j][i];
   __syncthreads();
   for (int e = threadIdx.x; e < window * 16 * NB; e += 64 * NW) {
     const int m = e / (16 * NB), c = e % (16 * NB);
-    const int r = rows_s[m];
+    const int r = sh.rows[m];
     if (r < 0 || col0 + c >= st.max_rank) continue;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) v += part[w][m][c];
-    v *= scale_s[m];
-    t[(size_t)r * ldt + col0 + c] = v;
+    for (int w = 0; w < NW; ++w) v += sh.part[w][m][c];
+    v *= sh.scale[m];
+    p.t[(size_t)r * p.ldt + col0 + c] = v;
   }
 }
 
-// ---- the wide product with the adapters' part -----------------------------------------------------------------------
+template <int NB, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW) void narrow_kernel(NarrowArgs p) {
+  __shared__ __align__(16) NarrowShared<NB, NW, VEC> sh;
+  narrow_block<NB, NW, VEC>(p, blockIdx.x, blockIdx.y, sh);
+}
+
+// ---- the wide product -----------------------------------------------------------------------
 struct WideArgs {
   const float *x; int ldx;       // rows x K
   const float *w; int ldw;       // NN: K x C, else C x K
@@ -336,35 +355,38 @@ struct WideArgs {
 
 // One workgroup per tile of 16 * MB rows and 16 * NB columns.  Its NW waves take steps of 32 of the inner dimension in turn
 // (no wave needs what another loads, so there is no barrier: a wave waits for its own piece of LDS) and add up through LDS
-// in a fixed order.  The columns of a lane are neighbours: block j of the tile holds columns NB * l + j.  The adapters' part
-// follows in the same way, the runs of equal adapters taken in turn by the waves: a run's product with its rows of the stack
-// is added to the run's rows only.
-// 256 rows, 2048 -> 2048, 40 adapters of rank 16 (32x64 tiles): 24.5 us, of which some 13 are splitting and multiplying (9
-// and 6 at full rate, hardly overlapped), 4 the adapters' part, 7 start and end; 88 TFLOP/s of float products.  One row:
-// 7.8 us for 16.8 MB of weights, three quarters of it the latencies of a kernel of dependent loads.  Loads straight into
-// the registers' layout (16 bytes of another row per lane) cap at 9 TB/s from the L2: 33 us for those 256 rows.
-template <int MB, int NB, int NW, bool NN, bool VEC>
-__global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
+// in a fixed order.  The columns of a lane are neighbours: block j of the tile holds columns NB * l + j.
+// FN > 0: the narrow product (FN: its NB) runs in the same launch, in the workgroups in front; the adapters' part, the
+// activation and the derivative below follow in a launch of their own, finish_kernel.  Three launches' chains of dependent
+// loads become two: one frame of 2048 -> 2048 10.4 us (narrow, then wide with the adapters' part: 12.9), 64 rows of 1024 ->
+// 1483 10.9 (16.1), 256 rows of 2048 -> 2048 with their plan 30.1 (35.0; 1 us more with the narrow product's workgroups behind
+// the tiles', 3 with 4 rows in each instead of one).
+// 256 rows, 2048 -> 2048 alone (32x64 tiles): 20 us, of which some 13 are splitting and multiplying (9 and 6 at full rate,
+// hardly overlapped), 7 start and end; 107 TFLOP/s of float products.  One row: 7.2 us for 16.8 MB of weights, three quarters
+// of it the latencies of a kernel of dependent loads.  Loads straight into the registers' layout (16 bytes of another row
+// per lane) cap at 9 TB/s from the L2: 33 us for those 256 rows.
+template <int MB, int NB, int NW, bool NN, bool VEC, int FN>
+__global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p, NarrowArgs narrow, int windows, int narrow_blocks) {
   constexpr int BM = 16 * MB, BN = 16 * NB, STAGED = NN ? BM : BM + BN;
   constexpr int SHARED = VEC && STAGED * 32 > BM * BN ? STAGED * 32 : BM * BN;
-  __shared__ __align__(16) float stage_s[NW * SHARED];  // a wave's rows of a step; at the end its sums
+  using Narrow = NarrowShared<FN ? FN : 1, NW, VEC>;
+  constexpr int BYTES = NW * SHARED * 4;
+  __shared__ __align__(16) char shared_s[FN && (int)sizeof(Narrow) > BYTES ? (int)sizeof(Narrow) : BYTES];
+  if (FN && (int)blockIdx.x < narrow_blocks)
+    return narrow_block<FN ? FN : 1, NW, VEC>(narrow, blockIdx.x % windows, blockIdx.x / windows,
+                                              *reinterpret_cast<Narrow *>(shared_s));
+  float *stage_s = reinterpret_cast<float *>(shared_s);  // a wave's rows of a step; at the end its sums
   float (*part)[BM][BN] = reinterpret_cast<float (*)[BM][BN]>(stage_s);
-  __shared__ int rows_s[BM];
   static_assert(64 * NW % BN == 0, "a thread finishes one column");
   // tiles of the same columns run on one of the 8 dies, so that a piece of W comes into one L2 only
-  const int die = blockIdx.x & 7, local = blockIdx.x >> 3;
+  const int block = blockIdx.x - (FN ? narrow_blocks : 0), die = block & 7, local = block >> 3;
   const int tile_n = die + 8 * (local / p.tiles_m), tile_m = local % p.tiles_m;
   if (tile_n >= p.tiles_n) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, q = lane >> 4;
   const int m0 = tile_m * BM, n0 = tile_n * BN, c0 = n0 + NB * l15;
-  const int row = lane < BM ? row_of(p.order, m0 + lane, p.N) : -1;
-  int my_row[MB];
   const float *xr[MB];
 #pragma unroll
-  for (int b = 0; b < MB; ++b) {
-    my_row[b] = __shfl(row, 16 * b + l15, 64);
-    xr[b] = p.x + (size_t)max(my_row[b], 0) * p.ldx;
-  }
+  for (int b = 0; b < MB; ++b) xr[b] = p.x + (size_t)min(m0 + 16 * b + l15, p.N - 1) * p.ldx;
   v4f acc[MB][NB];
 #pragma unroll
   for (int b = 0; b < MB; ++b)
@@ -405,27 +427,15 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
       for (int m = 0; m < MB; ++m) acc[m][j] = mfma6(fa[m], fb, acc[m][j]);
     }
   };
-  if (wave == 0 && lane < BM) rows_s[lane] = row;
   const int my_c = n0 + threadIdx.x % BN;
   const float my_bias = p.bias && my_c < p.C ? p.bias[my_c] : 0.f;  // for the end; asked for now
-  // the runs of equal adapters in the tile, and where the first that this wave takes has its rows of the stack: asked for
-  // now, used behind the product
-  Runs runs = {0, 0};
-  int first_lo = 0, first_rank = 0;
-  if (p.t) {
-    const int g = adapter_of(p.row_adapter, p.st.num, row);
-    runs = find_runs(g, lane);
-    unsigned long long left = runs.starts;
-    for (int i = 0; i < wave && left; ++i) left &= left - 1ull;
-    if (left) stack_rows(p.st, __shfl(g, __builtin_ctzll(left), 64), &first_lo, &first_rank);
-  }
   constexpr int D = 32 * NW;
   int k0 = 32 * wave;
   if (VEC && k0 + 32 <= p.K) {
     float *piece = stage_s + wave * STAGED * 32;
     const float *sx[2 * MB], *sw[2 * NB];
 #pragma unroll
-    for (int i = 0; i < 2 * MB; ++i) sx[i] = p.x + (size_t)max(__shfl(row, 8 * i + (lane >> 3), 64), 0) * p.ldx;
+    for (int i = 0; i < 2 * MB; ++i) sx[i] = p.x + (size_t)min(m0 + 8 * i + (lane >> 3), p.N - 1) * p.ldx;
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) {
       const int r = 8 * i + (lane >> 3);  // piece row 16 j + l: row NB l + j of the tile's part of W
@@ -470,61 +480,14 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
     multiply(rest);
   }
 
-  if (p.t) {
-    int turn = 0;
-    for (unsigned long long left = runs.starts; left; left &= left - 1ull, ++turn) {
-      if (turn % NW != wave) continue;
-      const int s = __builtin_ctzll(left);
-      const unsigned long long mask = run_mask(runs, s);
-      int lo = first_lo, rank = first_rank;
-      if (turn >= NW) stack_rows(p.st, adapter_of(p.row_adapter, p.st.num, __shfl(row, s, 64)), &lo, &rank);
-      v4f d[MB][NB];
-#pragma unroll
-      for (int m = 0; m < MB; ++m)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) d[m][j] = (v4f){0.f, 0.f, 0.f, 0.f};
-      for (int k0 = 0; k0 < rank; k0 += 32) {
-        float b[NB][8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int k = k0 + inner(q, e);
-          float v[NB] = {};
-          if (k < rank) load_cols<NB, VEC>(p.side + (size_t)(lo + k) * p.ldside, c0, p.C, v);
-#pragma unroll
-          for (int j = 0; j < NB; ++j) b[j][e] = v[j];
-        }
-        Frag fa[MB];
-#pragma unroll
-        for (int m = 0; m < MB; ++m) {
-          float a[8];
-          load_row8<VEC>(p.t + (size_t)max(my_row[m], 0) * p.ldt + k0, q, rank - k0, a);
-          fa[m] = split8(a);
-        }
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          const Frag fb = split8(b[j]);
-#pragma unroll
-          for (int m = 0; m < MB; ++m) d[m][j] = mfma6(fa[m], fb, d[m][j]);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < MB; ++m)
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if ((mask >> (16 * m + 4 * q + i)) & 1ull) acc[m][j][i] += d[m][j][i];
-    }
-  }
-
   __syncthreads();  // (the pieces of LDS have been read: now they take the sums)
   constexpr int EACH = BM * BN / (64 * NW) > 0 ? BM * BN / (64 * NW) : 1;
   float y[EACH];
   if (p.y) {
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-      const int m = (threadIdx.x + 64 * NW * i) / BN, r = m < BM ? rows_s[m] : -1;
-      y[i] = r >= 0 && my_c < p.C ? p.y[(size_t)r * p.ldy + my_c] : 0.f;
+      const int m = (threadIdx.x + 64 * NW * i) / BN;
+      y[i] = m < BM && m0 + m < p.N && my_c < p.C ? p.y[(size_t)(m0 + m) * p.ldy + my_c] : 0.f;
     }
   }
 #pragma unroll
@@ -536,16 +499,71 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const int m = (threadIdx.x + 64 * NW * i) / BN, r = m < BM ? rows_s[m] : -1;
-    if (r < 0 || my_c >= p.C) continue;
+    const int m = (threadIdx.x + 64 * NW * i) / BN;
+    if (m >= BM || m0 + m >= p.N || my_c >= p.C) continue;
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) sum += part[w][m][threadIdx.x % BN];
     float v = my_bias + sum;
     if (p.act == KH_ACT_SIGMOID) v = kh::sigmoidf(v);
     if (p.y) v = v * y[i] * (1.f - y[i]);
-    p.out[(size_t)r * p.ldout + my_c] = v;
+    p.out[(size_t)(m0 + m) * p.ldout + my_c] = v;
   }
+}
+
+// What these tiles leave to do: out += t * side of each row's adapter, then the activation or the derivative below.  A wave
+// has 64 columns of a row; CHUNK rows of the stack are on their way at a time.  256 rows of rank 16: 4.9 us (four columns a
+// lane, a quarter of the waves: 6.8 us; 64 rows of ranks up to 32: 4.4 and 14.0).
+struct FinishArgs {
+  int N, C;
+  const float *t; int ldt;
+  const float *side; int ldside;
+  Stack st;
+  const int32_t *row_adapter;
+  const float *y; int ldy;
+  int act;
+  float *out; int ldout;
+  __host__ __device__ long long units() const { return (long long)N * ((C + 63) / 64); }
+};
+template <int CHUNK>
+__device__ __forceinline__ void finish_unit(const FinishArgs &p, long long unit, int lane) {
+  const int col_units = (p.C + 63) / 64, r = (int)(unit / col_units), c = (int)(unit % col_units) * 64 + lane;
+  const int cc = min(c, p.C - 1);
+  float *out = p.out + (size_t)r * p.ldout + cc;
+  const float *t = p.t + (size_t)r * p.ldt;
+  const float raw = *out, y = p.y ? p.y[(size_t)r * p.ldy + cc] : 0.f;
+  const float first = lane < CHUNK && lane < p.st.max_rank ? t[lane] : 0.f;
+  const int g = __builtin_amdgcn_readfirstlane(adapter_of(p.row_adapter, p.st.num, r));
+  float sum = 0.f;
+  if (g >= 0) {
+    int lo, rank;
+    stack_rows(p.st, g, &lo, &rank);
+    const float *side = p.side + (size_t)lo * p.ldside + cc;
+    for (int k0 = 0; k0 < rank; k0 += CHUNK) {
+      const float a = k0 == 0 ? first : lane < CHUNK && k0 + lane < rank ? t[k0 + lane] : 0.f;
+      float b[CHUNK];
+#pragma unroll
+      for (int k = 0; k < CHUNK; ++k) b[k] = side[(size_t)min(k0 + k, rank - 1) * p.ldside];
+#pragma unroll
+      for (int k = 0; k < CHUNK; ++k)
+        if (k0 + k < rank) sum = fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), k)), b[k], sum);
+    }
+  }
+  float v = raw + sum;
+  if (p.act == KH_ACT_SIGMOID) v = kh::sigmoidf(v);
+  if (p.y) v = v * y * (1.f - y);
+  if (c < p.C) *out = v;
+}
+template <int CHUNK>
+__global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long units = p.units();
+  for (long long unit = 4ll * blockIdx.x + wave; unit < units; unit += 4ll * gridDim.x) finish_unit<CHUNK>(p, unit, lane);
+}
+void launch_finish(hipStream_t st, const FinishArgs &p) {
+  const unsigned blocks = (unsigned)std::min((p.units() + 3) / 4, 1ll << 20);
+  if (p.st.max_rank <= 16) finish_kernel<16><<<blocks, 256, 0, st>>>(p);
+  else finish_kernel<32><<<blocks, 256, 0, st>>>(p);
 }
 
 // ---- the wide product, tiles through LDS ----------------------------------------------------------------------------
@@ -825,8 +843,15 @@ struct GradArgs {
 };
 template <int MB, int NB, int NW, bool VEC>
 __global__ __launch_bounds__(64 * NW) void grad_kernel(GradArgs down, GradArgs up, int N, Stack st, const int32_t *order,
-                                                       const int32_t *row_begin, int col_tiles, int rank_blocks) {
+                                                       const int32_t *row_begin, int col_tiles, int rank_blocks, FinishArgs rest) {
   __shared__ float part[NW > 1 ? NW : 1][16 * MB][16 * NB];
+  if (blockIdx.y >= 2u * rank_blocks) {
+    const long long units = rest.units(), step = (long long)gridDim.x * (gridDim.y - 2 * rank_blocks) * NW;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (long long unit = ((long long)(blockIdx.y - 2 * rank_blocks) * gridDim.x + blockIdx.x) * NW + wave; unit < units; unit += step)
+      finish_unit<16 * MB>(rest, unit, threadIdx.x & 63);
+    return;
+  }
   const bool is_up = blockIdx.y >= (unsigned)rank_blocks;
   const GradArgs &p = is_up ? up : down;
   const int k_base = (blockIdx.y - (is_up ? rank_blocks : 0)) * 16 * MB;
@@ -898,22 +923,23 @@ __global__ __launch_bounds__(64 * NW) void grad_kernel(GradArgs down, GradArgs u
 }
 template <int MB, int NW, bool VEC>
 void launch_grad(hipStream_t st, const GradArgs &down, const GradArgs &up, int N, const Stack &stack, const int32_t *order,
-                 const int32_t *row_begin, int col_tiles) {
+                 const int32_t *row_begin, int col_tiles, const FinishArgs &rest) {
   const int rank_blocks = (stack.max_rank + 16 * MB - 1) / (16 * MB);
-  const dim3 grid((unsigned)col_tiles * stack.num, 2 * rank_blocks);
-  grad_kernel<MB, 2, NW, VEC><<<grid, 64 * NW, 0, st>>>(down, up, N, stack, order, row_begin, col_tiles, rank_blocks);
+  const long long x = (long long)col_tiles * stack.num, more = (rest.units() + x * NW - 1) / (x * NW);
+  const dim3 grid((unsigned)x, 2 * rank_blocks + (unsigned)std::min(more, 60000ll));
+  grad_kernel<MB, 2, NW, VEC><<<grid, 64 * NW, 0, st>>>(down, up, N, stack, order, row_begin, col_tiles, rank_blocks, rest);
 }
 template <bool VEC>
 void launch_grads(hipStream_t st, const GradArgs &down, const GradArgs &up, int N, const Stack &stack, const int32_t *order,
-                  const int32_t *row_begin, int col_tiles) {
+                  const int32_t *row_begin, int col_tiles, const FinishArgs &rest) {
   // one wave for adapters of few rows
   const bool few = N <= 64 * (long long)stack.num;
   if (stack.max_rank <= 16) {
-    if (few) launch_grad<1, 1, VEC>(st, down, up, N, stack, order, row_begin, col_tiles);
-    else launch_grad<1, 8, VEC>(st, down, up, N, stack, order, row_begin, col_tiles);
+    if (few) launch_grad<1, 1, VEC>(st, down, up, N, stack, order, row_begin, col_tiles, rest);
+    else launch_grad<1, 8, VEC>(st, down, up, N, stack, order, row_begin, col_tiles, rest);
   } else {
-    if (few) launch_grad<2, 1, VEC>(st, down, up, N, stack, order, row_begin, col_tiles);
-    else launch_grad<2, 8, VEC>(st, down, up, N, stack, order, row_begin, col_tiles);
+    if (few) launch_grad<2, 1, VEC>(st, down, up, N, stack, order, row_begin, col_tiles, rest);
+    else launch_grad<2, 8, VEC>(st, down, up, N, stack, order, row_begin, col_tiles, rest);
   }
 }
 
@@ -925,26 +951,33 @@ Stack stack_of(const khAdapters &ad) {
   return st;
 }
 
-template <bool VEC>
-void launch_narrow(hipStream_t st, const float *x, int ldx, int N, int K, const float *side, int ldside, const Stack &stack,
-                   const int32_t *row_adapter, const int32_t *order, float *t, int ldt) {
+int narrow_window(int N) {
   // windows of 16 rows fill the matrix instruction; below 256 of them (one per compute unit) smaller ones are faster
   int window = 16;
   while (window > 1 && (N + window - 1) / window < 256) window /= 2;
-  const int nb = stack.max_rank <= 16 ? 1 : 2;
-  const dim3 grid((N + window - 1) / window, (stack.max_rank + 16 * nb - 1) / (16 * nb));
-  if (nb == 1)
-    narrow_kernel<1, 8, VEC><<<grid, 512, 0, st>>>(x, ldx, N, K, side, ldside, stack, row_adapter, order, window, t, ldt);
-  else
-    narrow_kernel<2, 8, VEC><<<grid, 512, 0, st>>>(x, ldx, N, K, side, ldside, stack, row_adapter, order, window, t, ldt);
+  return window;
+}
+template <bool VEC>
+void launch_narrow(hipStream_t st, const NarrowArgs &p) {
+  const int nb = p.st.max_rank <= 16 ? 1 : 2;
+  const dim3 grid((p.N + p.window - 1) / p.window, (p.st.max_rank + 16 * nb - 1) / (16 * nb));
+  if (nb == 1) narrow_kernel<1, 8, VEC><<<grid, 512, 0, st>>>(p);
+  else narrow_kernel<2, 8, VEC><<<grid, 512, 0, st>>>(p);
 }
 
 template <int MB, int NB, int NW, bool NN, bool VEC>
-void launch_wide_tile(hipStream_t st, WideArgs p) {
+void launch_wide_tile(hipStream_t st, WideArgs p, const NarrowArgs &narrow, FinishArgs *rest) {
   p.tiles_m = (p.N + 16 * MB - 1) / (16 * MB);
   p.tiles_n = (p.C + 16 * NB - 1) / (16 * NB);
   const unsigned blocks = 8u * ((p.tiles_n + 7) / 8) * (unsigned)p.tiles_m;
-  wide_kernel<MB, NB, NW, NN, VEC><<<blocks, 64 * NW, 0, st>>>(p);
+  if (p.t == nullptr) return wide_kernel<MB, NB, NW, NN, VEC, 0><<<blocks, 64 * NW, 0, st>>>(p, narrow, 0, 0);
+  *rest = {p.N, p.C, p.t, p.ldt, p.side, p.ldside, p.st, p.row_adapter, p.y, p.ldy, p.act, p.out, p.ldout};
+  p.y = nullptr, p.act = KH_ACT_NONE;
+  const int fn = p.st.max_rank <= 16 ? 1 : 2, windows = (p.N + narrow.window - 1) / narrow.window;
+  // (a multiple of 8, so that the tiles still meet their dies; the blocks too many are behind the last rank column)
+  const int narrow_blocks = (windows * ((p.st.max_rank + 16 * fn - 1) / (16 * fn)) + 7) / 8 * 8;
+  if (fn == 1) wide_kernel<MB, NB, NW, NN, VEC, 1><<<narrow_blocks + blocks, 64 * NW, 0, st>>>(p, narrow, windows, narrow_blocks);
+  else wide_kernel<MB, NB, NW, NN, VEC, 2><<<narrow_blocks + blocks, 64 * NW, 0, st>>>(p, narrow, windows, narrow_blocks);
 }
 template <int WM, int WN, int MB, int NB, bool NN, bool VEC>
 void launch_tiled(hipStream_t st, WideArgs p) {
@@ -959,7 +992,7 @@ void launch_tiled(hipStream_t st, WideArgs p) {
 // 31, 64x128 64); 1024 rows 64x128 68 (32x64 74, 128x128 93); 2048 rows 128x128 106 (64x128 113, 256x128 156); 4096 rows
 // 256x128 176 (128x128 197).
 template <bool NN, bool VEC>
-void launch_wide(hipStream_t st, const WideArgs &p) {
+void launch_wide(hipStream_t st, const WideArgs &p, const NarrowArgs &narrow, FinishArgs *rest) {
   static const struct { int rows, cols, round; } kTiles[] = {{16, 16, 7}, {16, 32, 8}, {32, 64, 18}, {64, 128, 66}, {128, 128, 95}, {256, 128, 170}};
   // (hipK_gemm_row_invariant: the tiled kernels only, which sum an element in the same order whatever their tile)
   const int first = kh::gemm_row_invariant() ? 3 : 0;
@@ -970,10 +1003,11 @@ void launch_wide(hipStream_t st, const WideArgs &p) {
     const long long cost = (tiles + 255) / 256 * kTiles[i].round;
     if (i == first || cost < least) best = i, least = cost;
   }
+  if (best > 2 && p.t) launch_narrow<VEC>(st, narrow);
   switch (best) {
-    case 0: return launch_wide_tile<1, 1, 8, NN, VEC>(st, p);
-    case 1: return launch_wide_tile<1, 2, 16, NN, VEC>(st, p);
-    case 2: return launch_wide_tile<2, 4, 8, NN, VEC>(st, p);
+    case 0: return launch_wide_tile<1, 1, 8, NN, VEC>(st, p, narrow, rest);
+    case 1: return launch_wide_tile<1, 2, 16, NN, VEC>(st, p, narrow, rest);
+    case 2: return launch_wide_tile<2, 4, 8, NN, VEC>(st, p, narrow, rest);
     case 3: return launch_tiled<2, 4, 1, 1, NN, VEC>(st, p);
     case 4: return launch_tiled<4, 2, 1, 2, NN, VEC>(st, p);
     default: return launch_tiled<4, 2, 2, 2, NN, VEC>(st, p);
@@ -1036,16 +1070,17 @@ KH_EXPORT int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, 
   const Stack stack = stack_of(*ad);
   const bool vec = vec_ok(in, ldin) && vec_ok(W, ldw) && (ad->num == 0 || (vec_ok(ad->down, ad->lddown) &&
                    vec_ok(ad->up, ad->ldup) && vec_ok(t, ldt)));
-  if (ad->num > 0) {
-    if (vec) launch_narrow<true>(st, in, ldin, N, I, ad->down, ad->lddown, stack, row_adapter, order, t, ldt);
-    else launch_narrow<false>(st, in, ldin, N, I, ad->down, ad->lddown, stack, row_adapter, order, t, ldt);
-    rc = kh::launch_status();
-    if (rc != KH_OK) return rc;
-  }
+  const NarrowArgs na = {in, ldin, N, I, ad->down, ad->lddown, stack, row_adapter, order, narrow_window(N), t, ldt};
   WideArgs p = {in, ldin, W, ldw, N, I, O, bias, ad->num > 0 ? t : nullptr, ldt, ad->up, ad->ldup, stack, row_adapter, order,
                 nullptr, 0, act, out, ldout, 0, 0};
-  if (vec) launch_wide<false, true>(st, p);
-  else launch_wide<false, false>(st, p);
+  FinishArgs rest = {};
+  if (vec) launch_wide<false, true>(st, p, na, &rest);
+  else launch_wide<false, false>(st, p, na, &rest);
+  if (rest.N > 0) {
+    rc = kh::launch_status();
+    if (rc != KH_OK) return rc;
+    launch_finish(st, rest);
+  }
   rc = kh::launch_status();
   if (rc != KH_OK || act != KH_ACT_SOFTMAX) return rc;
   const MatrixDim d = {N, O, ldout};
@@ -1062,6 +1097,8 @@ KH_EXPORT int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t 
   int rc = check_adapters(ad, row_adapter, N, I, O);
   if (rc != KH_OK) return rc;
   const bool grads = ad->num > 0 && (gdown != nullptr || gup != nullptr);
+  const int cols = grads && ad->rows > 0 ? std::max(gdown != nullptr ? I : 0, gup != nullptr ? O : 0) : 0;
+  const int col_tiles = (cols + 31) / 32;
   KH_REQUIRE(N == 0 || O == 0 || (e != nullptr && lde >= O));
   KH_REQUIRE(eout == nullptr || (W != nullptr && ldw >= I && ldeout >= I && eout != e && eout != in));
   KH_REQUIRE(eout == nullptr || y == nullptr || ldy >= I);
@@ -1069,39 +1106,41 @@ KH_EXPORT int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t 
   KH_REQUIRE(!grads || (row_begin != nullptr && (N == 0 || order != nullptr)));
   KH_REQUIRE(gdown == nullptr || (ldgdown >= I && (N == 0 || (in != nullptr && ldin >= I))));
   KH_REQUIRE(gup == nullptr || (ldgup >= O && (N == 0 || (t != nullptr && ldt >= ad->max_rank))));
+  if ((long long)col_tiles * ad->num > 0x7fffffLL) {  // (workgroups of up to 512: the grid counts threads in 32 bits)
+    snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "gradients of %d adapters of %d columns: too many", ad->num, cols);
+    return KH_ERR_TOO_LARGE;
+  }
   KH_CHECK_INIT();
   rc = check_device();
   if (rc != KH_OK) return rc;
   hipStream_t st = kh::pick(s);
   const Stack stack = stack_of(*ad);
-  if (ad->num > 0 && N > 0) {
-    if (vec_ok(e, lde) && vec_ok(ad->up, ad->ldup))
-      launch_narrow<true>(st, e, lde, N, O, ad->up, ad->ldup, stack, row_adapter, order, u, ldu);
-    else launch_narrow<false>(st, e, lde, N, O, ad->up, ad->ldup, stack, row_adapter, order, u, ldu);
+  const NarrowArgs na = {e, lde, N, O, ad->up, ad->ldup, stack, row_adapter, order, narrow_window(N), u, ldu};
+  if (ad->num > 0 && N > 0 && (eout == nullptr || I == 0)) {
+    if (vec_ok(e, lde) && vec_ok(ad->up, ad->ldup)) launch_narrow<true>(st, na);
+    else launch_narrow<false>(st, na);
     rc = kh::launch_status();
     if (rc != KH_OK) return rc;
   }
+  FinishArgs rest = {};
   if (eout != nullptr && N > 0 && I > 0) {
     WideArgs p = {e, lde, W, ldw, N, O, I, nullptr, ad->num > 0 ? u : nullptr, ldu, ad->down, ad->lddown, stack, row_adapter,
                   order, y, ldy, KH_ACT_NONE, eout, ldeout, 0, 0};
-    const bool vec = vec_ok(e, lde) && vec_ok(W, ldw) && (ad->num == 0 || (vec_ok(ad->down, ad->lddown) && vec_ok(u, ldu)));
-    if (vec) launch_wide<true, true>(st, p);
-    else launch_wide<true, false>(st, p);
+    const bool vec = vec_ok(e, lde) && vec_ok(W, ldw) && (ad->num == 0 || (vec_ok(ad->down, ad->lddown) &&
+                     vec_ok(ad->up, ad->ldup) && vec_ok(u, ldu)));
+    if (vec) launch_wide<true, true>(st, p, na, &rest);
+    else launch_wide<true, false>(st, p, na, &rest);
     rc = kh::launch_status();
     if (rc != KH_OK) return rc;
   }
-  if (!grads || ad->rows == 0) return KH_OK;
+  if (cols == 0) {
+    if (rest.N > 0) launch_finish(st, rest);
+    return kh::launch_status();
+  }
   GradArgs gd = {u, ldu, in, ldin, gdown != nullptr ? I : 0, gdown, ldgdown};
   GradArgs gu = {t, ldt, e, lde, gup != nullptr ? O : 0, gup, ldgup};
-  const int cols = std::max(gd.C, gu.C);
-  if (cols == 0) return KH_OK;
-  const int col_tiles = (cols + 31) / 32;
-  if ((long long)col_tiles * ad->num > 0x7fffffffLL) {
-    snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "gradients of %d adapters of %d columns: too many", ad->num, cols);
-    return KH_ERR_TOO_LARGE;
-  }
   const bool vec = (gdown == nullptr || vec_ok(in, ldin)) && (gup == nullptr || vec_ok(e, lde));
-  if (vec) launch_grads<true>(st, gd, gu, N, stack, order, row_begin, col_tiles);
-  else launch_grads<false>(st, gd, gu, N, stack, order, row_begin, col_tiles);
+  if (vec) launch_grads<true>(st, gd, gu, N, stack, order, row_begin, col_tiles, rest);
+  else launch_grads<false>(st, gd, gu, N, stack, order, row_begin, col_tiles, rest);
   return kh::launch_status();
 }
