@@ -217,7 +217,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int32_t *row_adapter, 
 }
 
 // ---- the narrow product: t = s_g * x * side_g^T ----------------------------------------------------------------------
-// One workgroup per window of up to 16 rows and block of 16 * NB rank columns; its NW waves take steps of 32 of the
+// One workgroup per window of up to 16 rows and block of 16 * NB rank columns; its eight waves take steps of 32 of the
 // inner dimension in turn and add up through LDS in a fixed order.  A window of several adapters is gone through
 // once per run of equal adapters; only the run's rows are kept from a pass, so nothing of one row reaches another.  Bound
 // by reading x (4096 x 2048: 16 us, 2.1 TB/s) or, for few rows, by latency (1 to 64 rows: 6.3 us, with 4, 8 or 16 waves).
@@ -229,15 +229,18 @@ struct NarrowArgs {
   int window;
   float *t; int ldt;
 };
-template <int NB, int NW, bool VEC>
+constexpr int kNarrowWaves = 8;
+template <int NB, bool VEC>
 struct NarrowShared {
-  float stage[VEC ? NW * (16 + 16 * NB) * 32 : 4];
-  float part[NW][16][16 * NB + 4];
+  float stage[VEC ? kNarrowWaves * (16 + 16 * NB) * 32 : 4];
+  float part[kNarrowWaves][16][16 * NB + 4];
   int rows[16];
   float scale[16];
 };
-template <int NB, int NW, bool VEC>
-__device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, int block_y, NarrowShared<NB, NW, VEC> &sh) {
+// (waves behind the eighth, of a larger workgroup, have nothing to do: the order of the sums is the same in every kernel)
+template <int NB, bool VEC>
+__device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, int block_y, NarrowShared<NB, VEC> &sh) {
+  constexpr int NW = kNarrowWaves;
   const float *x = p.x, *side = p.side;
   const int ldx = p.ldx, N = p.N, K = p.K, lds = p.ldside, window = p.window;
   const Stack &st = p.st;
@@ -256,7 +259,7 @@ __device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, i
   v4f total[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) total[j] = (v4f){0.f, 0.f, 0.f, 0.f};
-  for (unsigned long long left = runs.starts; left; left &= left - 1ull) {
+  for (unsigned long long left = wave < NW ? runs.starts : 0ull; left; left &= left - 1ull) {
     const int s = __builtin_ctzll(left);
     const unsigned long long mask = run_mask(runs, s);
     int lo, rank;
@@ -314,12 +317,14 @@ __device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, i
       for (int i = 0; i < 4; ++i)
         if ((mask >> (4 * q + i)) & 1ull && col0 + NB * l15 + j < rank) total[j][i] = acc[j][i];
   }
+  if (wave < NW) {
 #pragma unroll
-  for (int j = 0; j < NB; ++j)
+    for (int j = 0; j < NB; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sh.part[wave][4 * q + i][NB * l15 + j] = total[j][i];
+      for (int i = 0; i < 4; ++i) sh.part[wave][4 * q + i][NB * l15 + j] = total[j][i];
+  }
   __syncthreads();
-  for (int e = threadIdx.x; e < window * 16 * NB; e += 64 * NW) {
+  for (int e = threadIdx.x; e < window * 16 * NB; e += blockDim.x) {
     const int m = e / (16 * NB), c = e % (16 * NB);
     const int r = sh.rows[m];
     if (r < 0 || col0 + c >= st.max_rank) continue;
@@ -331,10 +336,10 @@ __device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, i
   }
 }
 
-template <int NB, int NW, bool VEC>
-__global__ __launch_bounds__(64 * NW) void narrow_kernel(NarrowArgs p) {
-  __shared__ __align__(16) NarrowShared<NB, NW, VEC> sh;
-  narrow_block<NB, NW, VEC>(p, blockIdx.x, blockIdx.y, sh);
+template <int NB, bool VEC>
+__global__ __launch_bounds__(64 * kNarrowWaves) void narrow_kernel(NarrowArgs p) {
+  __shared__ __align__(16) NarrowShared<NB, VEC> sh;
+  narrow_block<NB, VEC>(p, blockIdx.x, blockIdx.y, sh);
 }
 
 // ---- the wide product -----------------------------------------------------------------------
@@ -369,12 +374,11 @@ template <int MB, int NB, int NW, bool NN, bool VEC, int FN>
 __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p, NarrowArgs narrow, int windows, int narrow_blocks) {
   constexpr int BM = 16 * MB, BN = 16 * NB, STAGED = NN ? BM : BM + BN;
   constexpr int SHARED = VEC && STAGED * 32 > BM * BN ? STAGED * 32 : BM * BN;
-  using Narrow = NarrowShared<FN ? FN : 1, NW, VEC>;
+  using Narrow = NarrowShared<FN ? FN : 1, VEC>;
   constexpr int BYTES = NW * SHARED * 4;
   __shared__ __align__(16) char shared_s[FN && (int)sizeof(Narrow) > BYTES ? (int)sizeof(Narrow) : BYTES];
   if (FN && (int)blockIdx.x < narrow_blocks)
-    return narrow_block<FN ? FN : 1, NW, VEC>(narrow, blockIdx.x % windows, blockIdx.x / windows,
-                                              *reinterpret_cast<Narrow *>(shared_s));
+    return narrow_block<FN ? FN : 1, VEC>(narrow, blockIdx.x % windows, blockIdx.x / windows, *reinterpret_cast<Narrow *>(shared_s));
   float *stage_s = reinterpret_cast<float *>(shared_s);  // a wave's rows of a step; at the end its sums
   float (*part)[BM][BN] = reinterpret_cast<float (*)[BM][BN]>(stage_s);
   static_assert(64 * NW % BN == 0, "a thread finishes one column");
@@ -961,8 +965,8 @@ template <bool VEC>
 void launch_narrow(hipStream_t st, const NarrowArgs &p) {
   const int nb = p.st.max_rank <= 16 ? 1 : 2;
   const dim3 grid((p.N + p.window - 1) / p.window, (p.st.max_rank + 16 * nb - 1) / (16 * nb));
-  if (nb == 1) narrow_kernel<1, 8, VEC><<<grid, 512, 0, st>>>(p);
-  else narrow_kernel<2, 8, VEC><<<grid, 512, 0, st>>>(p);
+  if (nb == 1) narrow_kernel<1, VEC><<<grid, 64 * kNarrowWaves, 0, st>>>(p);
+  else narrow_kernel<2, VEC><<<grid, 64 * kNarrowWaves, 0, st>>>(p);
 }
 
 template <int MB, int NB, int NW, bool NN, bool VEC>

@@ -363,6 +363,17 @@ def test_broken_tables_stay_inside(hip):
     c.begin = begin
 
 
+def test_a_row_of_t_whoever_shares_the_call(hip):
+    """Other row counts take other tiles and other windows: a row's narrow product is summed in the same order in all."""
+    whole = Case(hip, 600, 1483, 1024, 9, 32, "shuffled", seed=21)
+    want = whole.run_forward(0)[1]
+    for rows in (1, 40, 64, 300):
+        c = Case(hip, 600, 1483, 1024, 9, 32, "shuffled", seed=21)
+        c.N, c.ids = rows, whole.ids[:rows]
+        c.x = whole.x[:rows]
+        assert np.array_equal(c.run_forward(0)[1], want[:rows])
+
+
 def test_same_bits_again(hip):
     c = Case(hip, 700, 300, 260, 11, 40, "shuffled", seed=12)
     a = c.run_forward(1, True)
