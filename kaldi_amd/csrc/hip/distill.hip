@@ -4,6 +4,8 @@
 // Both are bound by reading (and writing) the logits once.  A row is one workgroup's, whose threads hold up to kHold floats
 // of it each: up to 1024 * kHold = 20480 columns stay in registers between the maximum, the sum and the output, and longer
 // rows are gone through in such chunks.
+#include <algorithm>
+
 #include "common.h"
 
 namespace {
@@ -578,6 +580,8 @@ void launch_row_top_as(hipStream_t st, const float *mat, MatrixDim d, int K, int
   if constexpr (AHEAD) row_top_kernel<THREADS, VEC, true><<<rows < most ? rows : most, THREADS, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
   else row_top_kernel<THREADS, VEC, false><<<rows, THREADS, 0, st>>>(mat, d, K, idx, ldidx, val, ldval, lse);
 }
+// A grid counts its threads in 32 bits: more rows than this go in several launches.
+constexpr int kRowsAtOnce = 1 << 21;
 template <bool VEC>
 void launch_row_top(hipStream_t st, const float *mat, MatrixDim d, int K, int32_t *idx, int ldidx, float *val, int ldval,
                     float *lse) {
@@ -614,9 +618,16 @@ KH_EXPORT int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t 
   if (rc != KH_OK) return rc;
   if (d.rows == 0) return KH_OK;
   hipStream_t st = kh::pick(s);
-  if (kh::aligned16(mat) && d.stride % 4 == 0) launch_row_top<true>(st, mat, d, K, idx, ldidx, val, ldval, lse);
-  else launch_row_top<false>(st, mat, d, K, idx, ldidx, val, ldval, lse);
-  return kh::launch_status();
+  const bool vec = kh::aligned16(mat) && d.stride % 4 == 0;
+  for (size_t r = 0; r < (size_t)d.rows; r += kRowsAtOnce) {
+    const MatrixDim part = {std::min(d.rows - (int)r, kRowsAtOnce), d.cols, d.stride};
+    float *l = lse ? lse + r : nullptr;
+    if (vec) launch_row_top<true>(st, mat + r * d.stride, part, K, idx + r * ldidx, ldidx, val + r * ldval, ldval, l);
+    else launch_row_top<false>(st, mat + r * d.stride, part, K, idx + r * ldidx, ldidx, val + r * ldval, ldval, l);
+    rc = kh::launch_status();
+    if (rc != KH_OK) return rc;
+  }
+  return KH_OK;
 }
 
 KH_EXPORT int hipF_distill_eval(khStream_t s, const float *x, MatrixDim d, const int32_t *idx, int32_t ldidx,
@@ -637,16 +648,22 @@ KH_EXPORT int hipF_distill_eval(khStream_t s, const float *x, MatrixDim d, const
   if (rc != KH_OK) return rc;
   if (d.rows == 0) return KH_OK;
   hipStream_t st = kh::pick(s);
-  DistillArgs p = {x, d, idx, ldidx, val, ldval, K, label, weight, temperature, hard_weight,
-                   exp_scale(hard_weight == 1.f ? 1.0 : 1.0 / (double)temperature), diff, lddiff, row_loss};
   const bool vec = kh::aligned16(x) && d.stride % 4 == 0 && (diff == nullptr || (kh::aligned16(diff) && lddiff % 4 == 0));
   const bool both = hard_weight > 0.f && hard_weight < 1.f && temperature != 1.f;
-  if (vec && both) launch_distill<true, true>(st, p);
-  else if (vec) launch_distill<true, false>(st, p);
-  else if (both) launch_distill<false, true>(st, p);
-  else launch_distill<false, false>(st, p);
-  rc = kh::launch_status();
-  if (rc != KH_OK || loss == nullptr) return rc;
+  for (size_t r = 0; r < (size_t)d.rows; r += kRowsAtOnce) {
+    const MatrixDim part = {std::min(d.rows - (int)r, kRowsAtOnce), d.cols, d.stride};
+    const DistillArgs p = {x + r * d.stride, part, idx + r * ldidx, ldidx, val + r * ldval, ldval, K, label ? label + r : nullptr,
+                           weight ? weight + r : nullptr, temperature, hard_weight,
+                           exp_scale(hard_weight == 1.f ? 1.0 : 1.0 / (double)temperature), diff ? diff + r * lddiff : nullptr, lddiff,
+                           row_loss ? row_loss + r : nullptr};
+    if (vec && both) launch_distill<true, true>(st, p);
+    else if (vec) launch_distill<true, false>(st, p);
+    else if (both) launch_distill<false, true>(st, p);
+    else launch_distill<false, false>(st, p);
+    rc = kh::launch_status();
+    if (rc != KH_OK) return rc;
+  }
+  if (loss == nullptr) return KH_OK;
   sum_rows_kernel<<<1, 256, 0, st>>>(row_loss, d.rows, loss);
   return kh::launch_status();
 }

@@ -348,3 +348,38 @@ def test_teacher_to_student(hip):
     h.call("hipF_softmax", None, q.ptr, q.ptr, q.dim)
     np.testing.assert_allclose(dx.numpy(), p.numpy() - q.numpy(), rtol=0, atol=2.0 ** -16)
     assert (row_loss.numpy() > 0).all()
+
+
+def test_more_rows_than_one_launch_takes(hip):
+    """Rows go in launches of 2^21: what the second one reads and writes lies behind the first one's.  Of the last rows, with
+    |x| <= 1, K = 2, T = 1: a probability is good to 2^-16 (above), the gradient, two of them, to 2^-15; a loss is at most five
+    logarithms of size <= 4, each weighed by a probability, so good to 5 * 4 * 2^-17 < 2^-12."""
+    R, C, K, n = 2 ** 21 + 3, 5, 2, 9
+    rs = np.random.RandomState(5)
+    x = rs.uniform(-1, 1, (R, C)).astype(f32)
+    dx, di, dv, dl = dev(hip, x, False), hip.DevMatrix(R, K, np.int32, False), hip.DevMatrix(R, K, f32, False), dev(hip, np.zeros((1, R), f32), False)
+    hip.call("hipF_row_top", None, dx.ptr, hip.MatrixDim(R, C, C), K, di.ptr, K, dv.ptr, K, dl.ptr)
+    idx, val = di.numpy(), dv.numpy()
+    assert np.array_equal(idx, np.argsort(-x, axis=1, kind="stable")[:, :K])
+    assert np.array_equal(val, np.take_along_axis(x, idx, 1))
+    lse = np.log(np.exp(x.astype(f64)).sum(1))
+    assert np.abs(dl.numpy()[0] - lse).max() <= 2.0 ** -17
+    label = rs.randint(0, C, R).astype(np.int32)
+    diff, row_loss = hip.DevMatrix(R, C, f32, False), dev(hip, np.zeros((1, R), f32), False)
+    loss = dev(hip, np.zeros((1, 2), f32), False)  # a double
+    dlabel = dev(hip, label[None], False)
+    student = np.roll(x, 1, 1)
+    ds = dev(hip, student, False)
+    hip.call("hipF_distill_eval", None, ds.ptr, hip.MatrixDim(R, C, C), di.ptr, K, dv.ptr, K, K, dlabel.ptr, None, 1.0, 0.5, diff.ptr, C,
+             row_loss.ptr, loss.ptr)
+    z = student[-n:].astype(f64)
+    lp = z - np.log(np.exp(z).sum(1, keepdims=True))
+    q = np.zeros_like(z)
+    v = val[-n:].astype(f64)
+    np.put_along_axis(q, idx[-n:], np.exp(v) / np.exp(v).sum(1, keepdims=True), 1)
+    hot = np.eye(C)[label[-n:]]
+    want = 0.5 * (q * (np.log(np.where(q > 0, q, 1)) - lp)).sum(1) - 0.5 * (hot * lp).sum(1)
+    got = row_loss.numpy()[0]
+    assert np.abs(got[-n:] - want).max() <= 2.0 ** -12
+    assert np.abs(diff.numpy()[-n:] - (np.exp(lp) - 0.5 * q - 0.5 * hot)).max() <= 2.0 ** -15
+    assert np.isclose(loss.numpy().view(f64)[0, 0], got.astype(f64).sum(), rtol=1e-9, atol=0)
