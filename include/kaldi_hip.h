@@ -483,7 +483,7 @@ typedef struct {
 /* Groups the N rows of a bunch by adapter: order[] lists the rows of adapter 0, then of adapter 1, ..., each in
  * ascending order, then the rows without one (row_adapter[r] outside [0, num)); adapter g's are
  * order[row_begin[g] .. row_begin[g+1]-1].  order: N, row_begin: num + 1 int32 on the device.  One bunch's grouping
- * serves every layer, forward and backward. */
+ * serves every layer, forward and backward.  num <= 2^21. */
 int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int32_t num, int32_t *order,
                         int32_t *row_begin);
 
@@ -496,7 +496,7 @@ int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int
  * together already (utterances, single frames).  The result does not depend on it beyond rounding (a row that a broken
  * order does not list may stay unwritten).  `t` is what
  * the backward pass needs; bias may be NULL.  out and t must not overlap an input.  Rows behind N and columns
- * behind O (max_rank) are left as they are.  Uses no library workspace: may be captured into a graph.  A row of t has
+ * behind O (max_rank) are left as they are.  N <= 2^26.  Uses no library workspace: may be captured into a graph.  A row of t has
  * the same bits whoever shares its call, and with hipK_gemm_row_invariant(1) so has a row of out.
  * Arithmetic: every float is taken as the sum of three bfloat16 numbers (24 bits of mantissa: exact) and a product
  * of two floats as the six largest of the nine part products, on the matrix cores with float sums; what is left out
@@ -516,7 +516,7 @@ int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, int32_t I,
  * order / row_begin: hipI32_adapter_plan of the same rows; order must be a permutation of 0 .. N-1 for the
  * gradients to be whole (an entry outside is skipped).  An adapter without rows gets a gradient of zeros; rows of the
  * stacks outside every adapter are left as they are.  Sums are taken in a fixed order: the same call gives the same
- * bits.  Outputs must not overlap an input.  The shared W is not updated here (hipF_affine_update). */
+ * bits.  Outputs must not overlap an input.  N <= 2^26, num * max(I, O) / 32 < 2^23 with gradients.  The shared W is not updated here (hipF_affine_update). */
 int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t I, const float *e, int32_t lde, const float *in,
                           int32_t ldin, const float *W, int32_t ldw, const khAdapters *ad, const int32_t *row_adapter,
                           const int32_t *order, const int32_t *row_begin, const float *t, int32_t ldt, float *u,
@@ -532,7 +532,8 @@ int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t I, const f
  * NaN above every number: idx[r,k] = column, val[r,k] = mat[r, idx[r,k]].  K beyond the row's length fills up with
  * idx -1, val -inf.  lse[r] = log(sum_c exp(mat[r,c])) (may be NULL; -inf for a row of -inf, NaN for
  * one that holds a NaN or +inf), so that val - lse are log-posteriors.  What hipF_find_row_max_id is for one
- * maximum; it makes a teacher's outputs small enough to keep.  Uses no library workspace. */
+ * maximum; it makes a teacher's outputs small enough to keep.  The outputs must not overlap mat.  Uses no library
+ * workspace. */
 int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t K, int32_t *idx, int32_t ldidx, float *val,
                  int32_t ldval, float *lse);
 

@@ -998,8 +998,9 @@ void launch_tiled(hipStream_t st, WideArgs p) {
 template <bool NN, bool VEC>
 void launch_wide(hipStream_t st, const WideArgs &p, const NarrowArgs &narrow, FinishArgs *rest) {
   static const struct { int rows, cols, round; } kTiles[] = {{16, 16, 7}, {16, 32, 8}, {32, 64, 18}, {64, 128, 66}, {128, 128, 95}, {256, 128, 170}};
-  // (hipK_gemm_row_invariant: the tiled kernels only, which sum an element in the same order whatever their tile)
-  const int first = kh::gemm_row_invariant() ? 3 : 0;
+  // (hipK_gemm_row_invariant: the tiled kernels only, which sum an element in the same order whatever their tile; so too where
+  // the small tiles' workgroups might be too many for a grid)
+  const int first = kh::gemm_row_invariant() || p.N > (1 << 20) ? 3 : 0;
   int best = first;
   long long least = 0;
   for (int i = first; i < 6; ++i) {
@@ -1018,8 +1019,16 @@ void launch_wide(hipStream_t st, const WideArgs &p, const NarrowArgs &narrow, Fi
   }
 }
 
+// A grid counts its threads in 32 bits: 2^26 rows in windows of 16 rows and 512 threads fill half of that.
+constexpr int kMaxRows = 1 << 26, kMaxAdapters = 1 << 21;
+int too_many(const char *what, int n, int most) {
+  snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "%d %s: at most %d", n, what, most);
+  return KH_ERR_TOO_LARGE;
+}
+
 int check_adapters(const khAdapters *ad, const int32_t *row_adapter, int32_t N, int32_t I, int32_t O) {
   KH_REQUIRE(ad != nullptr && ad->num >= 0);
+  if (N > kMaxRows) return too_many("rows", N, kMaxRows);
   if (ad->num == 0) return KH_OK;
   KH_REQUIRE(ad->max_rank >= 1 && ad->rows >= 0);
   if (ad->max_rank > KH_MAX_ADAPTER_RANK) {
@@ -1047,6 +1056,7 @@ KH_EXPORT int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int3
                                   int32_t *row_begin) {
   KH_REQUIRE(N >= 0 && num >= 0 && row_begin != nullptr);
   KH_REQUIRE(N == 0 || (row_adapter != nullptr && order != nullptr));
+  if (num > kMaxAdapters) return too_many("adapters", num, kMaxAdapters);  // (a workgroup of up to 1024 for each)
   KH_CHECK_INIT();
   int rc = check_device();
   if (rc != KH_OK) return rc;
@@ -1064,7 +1074,7 @@ KH_EXPORT int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, 
   int rc = check_adapters(ad, row_adapter, N, I, O);
   if (rc != KH_OK) return rc;
   KH_REQUIRE(N == 0 || (ldin >= I && ldw >= I && ldout >= O));
-  KH_REQUIRE(ad->num == 0 || N == 0 || (t != nullptr && ldt >= ad->max_rank));
+  KH_REQUIRE(ad->num == 0 || N == 0 || (t != nullptr && t != out && ldt >= ad->max_rank));
   KH_REQUIRE(N == 0 || O == 0 || (out != nullptr && out != in && (I == 0 || (in != nullptr && W != nullptr))));
   KH_CHECK_INIT();
   rc = check_device();
@@ -1105,7 +1115,7 @@ KH_EXPORT int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t 
   const int col_tiles = (cols + 31) / 32;
   KH_REQUIRE(N == 0 || O == 0 || (e != nullptr && lde >= O));
   KH_REQUIRE(eout == nullptr || (W != nullptr && ldw >= I && ldeout >= I && eout != e && eout != in));
-  KH_REQUIRE(eout == nullptr || y == nullptr || ldy >= I);
+  KH_REQUIRE(eout == nullptr || (eout != u && eout != y && (y == nullptr || ldy >= I)));
   KH_REQUIRE(ad->num == 0 || N == 0 || (u != nullptr && ldu >= ad->max_rank && u != t));
   KH_REQUIRE(!grads || (row_begin != nullptr && (N == 0 || order != nullptr)));
   KH_REQUIRE(gdown == nullptr || (ldgdown >= I && (N == 0 || (in != nullptr && ldin >= I))));

@@ -116,7 +116,8 @@ class Adapters {
                      const AdapterRows &rows, const CuMatrix<BaseFloat> *y, CuMatrix<BaseFloat> *out_err) {
     CuProfileScope p("Adapters::Backpropagate");
     Check(layer, in, rows);
-    KALDI_ASSERT(in_err.NumRows() == in.NumRows() && in_err.NumCols() == output_dim_ && t_.NumRows() == in.NumRows());
+    KALDI_ASSERT(in_err.NumRows() == in.NumRows() && in_err.NumCols() == output_dim_ && t_.NumRows() == in.NumRows() &&
+                 t_.NumCols() == max_rank_);
     KALDI_ASSERT(y == NULL || (y->NumRows() == in.NumRows() && y->NumCols() == input_dim_));
     if (out_err && (out_err->NumRows() != in.NumRows() || out_err->NumCols() != input_dim_))
       out_err->Resize(in.NumRows(), input_dim_);
@@ -164,12 +165,15 @@ class Adapters {
     if (output_dim <= 0 || input_dim <= 0 || static_cast<size_t>(scale.Dim()) != ranks.size())
       KALDI_ERR << "Adapters: " << ranks.size() << " ranks, " << scale.Dim() << " scales, " << input_dim << " -> " << output_dim;
     std::vector<BaseFloat> s(ranks.size());
-    for (size_t g = 0; g < s.size(); ++g) s[g] = scale(g);
+    int64 rows = 0;
+    for (size_t g = 0; g < s.size(); ++g) {
+      s[g] = scale(g);
+      rows += ranks[g];
+    }
+    if (down.NumRows() != rows || up.NumRows() != rows ||
+        (rows > 0 && (down.NumCols() != input_dim || up.NumCols() != output_dim)))
+      KALDI_ERR << "Adapters: stacks of " << down.NumRows() << " and " << up.NumRows() << " rows, the ranks add up to " << rows;
     Init(input_dim, output_dim, ranks, s);
-    if (down.NumRows() != down_.NumRows() || up.NumRows() != up_.NumRows() ||
-        (down.NumRows() > 0 && (down.NumCols() != input_dim || up.NumCols() != output_dim)))
-      KALDI_ERR << "Adapters: stacks of " << down.NumRows() << " and " << up.NumRows() << " rows, the ranks add up to "
-                << down_.NumRows();
     if (down.NumRows() > 0) {
       SetDown(down);
       SetUp(up);

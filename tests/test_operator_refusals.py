@@ -85,6 +85,25 @@ def test_distill_refuses(change):
     assert status("hipF_distill_eval", DISTILL, **change) == INVALID
 
 
+def test_outputs_over_each_other():
+    assert status("hipF_adapter_forward", FORWARD, t=2 * P) == INVALID
+    assert status("hipF_adapter_backward", BACKWARD, y=3 * P, ldy=32) == INVALID
+    assert status("hipF_adapter_backward", BACKWARD, eout=2 * P) == INVALID
+
+
+def test_too_many():
+    rows = 2 ** 26 + 1
+    assert status("hipF_adapter_forward", FORWARD, N=rows) == TOO_LARGE
+    assert b"67108865" in h.lib.hipK_error_string(TOO_LARGE)
+    assert status("hipF_adapter_backward", BACKWARD, N=rows) == TOO_LARGE
+    assert status("hipF_adapter_forward", FORWARD, N=rows, ad=adapters(num=0)) == TOO_LARGE
+    assert status("hipI32_adapter_plan", PLAN, num=2 ** 21 + 1) == TOO_LARGE
+    assert b"2097153" in h.lib.hipK_error_string(TOO_LARGE)
+    # one workgroup per adapter and 32 columns
+    assert status("hipF_adapter_backward", BACKWARD, ad=adapters(num=2 ** 22)) == TOO_LARGE
+    assert b"48 columns" in h.lib.hipK_error_string(TOO_LARGE)
+
+
 def test_k_too_large():
     big = h.MAX_TOP + 1
     assert status("hipF_row_top", TOP, K=big, ldidx=256, ldval=256) == TOO_LARGE
