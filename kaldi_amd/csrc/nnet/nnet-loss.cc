@@ -128,9 +128,9 @@ void Distill::Eval(const CuMatrix<BaseFloat> &net_out, const CuStlVector<int32> 
   KALDI_ASSERT(val.NumRows() == n && id.Dim() == static_cast<size_t>(n) * k);
   KALDI_ASSERT(label == NULL || static_cast<int32>(label->Dim()) == n);
   KALDI_ASSERT(weight == NULL || static_cast<int32>(weight->Dim()) == n);
-  if (n == 0) return;
   if (diff && diff != &net_out) diff->Resize(n, net_out.NumCols());
   row_loss_.Resize(n);
+  if (n == 0) return;
   CU_SAFE_CALL(hipF_distill_eval(S(), net_out.Data(), net_out.Dim(), id.Data(), k, val.Data(), val.Stride(), k,
                                  label ? label->Data() : NULL, weight ? weight->Data() : NULL, temperature_, hard_weight_,
                                  diff ? diff->Data() : NULL, diff ? diff->Stride() : 0, row_loss_.Data(), stats_.Loss()));
