@@ -101,7 +101,10 @@ if not os.path.exists(LIB_PATH):
         "kaldi_amd: %s is missing; the HIP device library must be built first "
         "(python -c 'import __graft_entry__ as g; g.build()').  There is no CPU fallback." % LIB_PATH)
 
-lib = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL)
+# Local: the symbols of the ROCm libraries behind this one must not take the place of those that torch brings along (a process
+# that imported torch afterwards ended in a double free).  Another library named in the environment is global, so that
+# libkaldi_nnet.so binds to it and not to the one beside itself.
+lib = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL if os.environ.get("KALDI_AMD_HIP_LIB") else ctypes.RTLD_LOCAL)
 PROTOS = parse_header()
 for _name, (_res, _args) in PROTOS.items():
     _fn = getattr(lib, _name)  # AttributeError here = header/library mismatch

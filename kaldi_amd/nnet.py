@@ -11,7 +11,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libk
 BIN_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "bin")
 if not os.path.exists(LIB_PATH):
     raise ImportError("kaldi_amd: %s is missing; build it first (__graft_entry__.build())" % LIB_PATH)
-lib = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL)
+lib = ctypes.CDLL(LIB_PATH)  # local, as in hip.py
 
 P, I, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
 _SIGS = {

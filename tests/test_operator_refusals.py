@@ -1,6 +1,9 @@
 """What the adapter, top-logit and distillation entry points refuse.  Arguments are checked before the device is looked for,
 so these run without a GPU: a refused call never reaches a kernel."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -102,6 +105,14 @@ def test_too_many():
     # one workgroup per adapter and 32 columns
     assert status("hipF_adapter_backward", BACKWARD, ad=adapters(num=2 ** 22)) == TOO_LARGE
     assert b"48 columns" in h.lib.hipK_error_string(TOO_LARGE)
+
+
+@pytest.mark.parametrize("first", ["kaldi_amd.hip", "kaldi_amd.nnet"])
+def test_torch_behind_the_library(first):
+    """A program that uses both, in this order, ends as it should."""
+    env = {k: v for k, v in os.environ.items() if k != "KALDI_AMD_HIP_LIB"}
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    assert subprocess.run([sys.executable, "-c", "import %s, torch" % first], env=env, cwd=root, timeout=300).returncode == 0
 
 
 def test_k_too_large():
