@@ -990,14 +990,15 @@ void launch_tiled(hipStream_t st, WideArgs p) {
   const unsigned blocks = 8u * (((unsigned)p.tiles_m * p.tiles_n + 7) / 8);
   tiled_kernel<WM, WN, MB, NB, NN, VEC><<<blocks, 512, 0, st>>>(p);
 }
-// Which kernel and tile.  The tiles of a product are worked off in rounds of one per compute unit; what a round takes was
-// measured with 2048 inner indices (us): 16 rows x 16 columns 7, 16 x 32 8, 32 x 64 18, 64 x 128 66, 128 x 128 95, 256 x 128
-// 170.  E.g. 2048 columns: 1 row 16x16 7 us (16x32 7.5, 32x64 16); 64 rows 16x32 8 (16x16 10, 32x64 17); 256 rows 32x64 18 (16x32
-// 31, 64x128 64); 1024 rows 64x128 68 (32x64 74, 128x128 93); 2048 rows 128x128 106 (64x128 113, 256x128 156); 4096 rows
-// 256x128 176 (128x128 197).
+// Which kernel and tile.  The tiles of a product are worked off in rounds of one per compute unit; what a round takes of a
+// whole call was fitted to calls of 1 to 4096 rows with adapters of rank 16, 512 to 2048 inner indices and columns (us): 16 rows
+// x 16 columns 7, 16 x 32 11, 32 x 64 21, 64 x 128 62, 128 x 128 95, 256 x 128 170; the choice is within 1.3 % of the fastest
+// tile on average, within 14 % at worst.  E.g. 2048 -> 2048: 1 row 16x16 10 us (16x32 10, 32x64 18); 64 rows 16x32 16 (16x16 16,
+// 32x64 20); 256 rows 32x64 28 (16x32 38, 64x128 66); 1024 rows 64x128 73 (32x64 85, 128x128 101); 2048 rows 128x128 114 (64x128
+// 121, 256x128 167); 4096 rows 256x128 193 (128x128 220).
 template <bool NN, bool VEC>
 void launch_wide(hipStream_t st, const WideArgs &p, const NarrowArgs &narrow, FinishArgs *rest) {
-  static const struct { int rows, cols, round; } kTiles[] = {{16, 16, 7}, {16, 32, 8}, {32, 64, 18}, {64, 128, 66}, {128, 128, 95}, {256, 128, 170}};
+  static const struct { int rows, cols, round; } kTiles[] = {{16, 16, 7}, {16, 32, 11}, {32, 64, 21}, {64, 128, 62}, {128, 128, 95}, {256, 128, 170}};
   // (hipK_gemm_row_invariant: the tiled kernels only, which sum an element in the same order whatever their tile; so too where
   // the small tiles' workgroups might be too many for a grid)
   const int first = kh::gemm_row_invariant() || p.N > (1 << 20) ? 3 : 0;

@@ -9,6 +9,8 @@ rounding is at most 2^-24 of a partial sum, and no partial sum exceeds the sum o
     |error| <= 2^-24 * M * (24 * ceil(K / 256) + 24 * ceil(rank / 32) + 16)
 
 Variants that sum K in one piece take K / 32 steps in a row: 24 * ceil(K / 32) in its place; the tests use that, the larger.
+With few rows the adapters' part is a chain of `rank` fused multiply-adds, one rounding each: up to 32 * ceil(rank / 32) in the
+place of 24 * ceil(rank / 32); the tests use that, the larger.
 """
 import ctypes
 
@@ -21,7 +23,7 @@ EPS = 2.0 ** -24
 
 
 def bound(K, rank=0):
-    return EPS * (24 * -(-K // 32) + 24 * -(-rank // 32) + 16)
+    return EPS * (24 * -(-K // 32) + 32 * -(-rank // 32) + 16)
 
 
 class Case:
@@ -147,7 +149,11 @@ SHAPES = [
     (1, 64, 64, 3, 16, "each"), (1, 1, 1, 1, 1, "each"), (3, 17, 33, 2, 5, "each"), (16, 16, 32, 1, 16, "segments"),
     (17, 130, 100, 7, 33, "each"), (64, 259, 440, 80, 32, "each"), (100, 2048, 1320, 5, 16, "shuffled"),
     (256, 1483, 1024, 40, 16, "shuffled"), (300, 512, 511, 3, 128, "segments"), (1000, 320, 256, 500, 7, "shuffled"),
-    (2100, 192, 130, 12, 64, "segments"), (4097, 257, 96, 9, 24, "shuffled")]
+    (2100, 192, 130, 12, 64, "segments"), (4097, 257, 96, 9, 24, "shuffled"),
+    # the other tiles, forward and backward
+    (60, 1483, 70, 9, 40, "each"), (50, 70, 1483, 9, 40, "shuffled"), (1000, 2048, 70, 12, 20, "shuffled"),
+    (1000, 50, 2048, 12, 20, "shuffled"), (2000, 2048, 40, 12, 33, "segments"), (2000, 40, 2048, 12, 33, "segments"),
+    (4000, 2048, 36, 12, 128, "shuffled"), (4000, 36, 2048, 12, 128, "shuffled")]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -209,6 +215,15 @@ def test_backward(hip, shape):
     c = Case(hip, *shape, seed=sum(shape[:5]) + 1)
     t = c.forward(0)[1].astype(f32)
     check_backward(c, t, with_y=shape[0] % 2 == 0)
+
+
+def test_more_rows_than_the_small_tiles_take(hip):
+    c = Case(hip, 2 ** 20 + 3, 6, 5, 3, 4, "segments", seed=14)
+    out, t = c.run_forward(0)
+    want, t64, mag, tmag = c.forward(0)
+    within(t, t64, bound(c.I) * tmag + 1e-37)
+    within(out, want, (bound(c.I, c.rank) + bound(c.I)) * mag)
+    check_backward(c, t)
 
 
 def test_backward_of_the_lowest_layer_and_of_frozen_adapters(hip):
