@@ -142,8 +142,9 @@ constexpr int kCap = 1024;  // candidates of a chunk, next to the KH_MAX_TOP of 
 
 // AHEAD false: a workgroup has one row, of one chunk; 64 registers, so that eight waves share a SIMD and hide each other's
 // loads (4096 rows of 9000, K 32: 36.7 us, 4.0 TB/s, what a plain sum of as much memory reads at).  AHEAD: rows of several
-// chunks; a workgroup takes one row after another and has the next chunk loaded into LDS while it works on one in
-// registers, a wave waiting for its own part only (256 rows of 70001, K 64: 24.9 us; short rows measure 44 us that way).
+// chunks of equal length; a workgroup takes one row after another and has the next chunk loaded into LDS while it works on one
+// in registers, a wave waiting for its own part only (256 rows of 70001, K 64: 24.1 us, 25.0 with whole chunks and a rest;
+// short rows measure 44 us that way).
 // A row's first chunk: its threads form G groups; a value that at least K groups' maxima reach is a lower bound of the
 // chunk's K-th largest, and where large values are spread over the row few more than K elements reach the best such value.
 // It is found by bisection to K .. 1.25 K groups, every wave for itself.  (Later chunks: the K-th largest so far.)  The
@@ -161,8 +162,10 @@ __global__ __launch_bounds__(THREADS, AHEAD ? 4 : THREADS == 64 ? 3 : 8) void ro
   __shared__ int count_s[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
+  // chunks of equal length
+  const int chunks = (d.cols + chunk - 1) / chunk, step = AHEAD && chunks > 1 ? ((d.cols + chunks - 1) / chunks + 3) & ~3 : chunk;
   if (AHEAD && blockIdx.x < (unsigned)d.rows && d.cols > 0)
-    load_chunk<THREADS, VEC>(mat + (size_t)blockIdx.x * d.stride, d.cols, ahead, tid, wave);
+    load_chunk<THREADS, VEC>(mat + (size_t)blockIdx.x * d.stride, min(d.cols, step), ahead, tid, wave);
   for (long long r = blockIdx.x; r < d.rows; r += gridDim.x) {
     const float *row = mat + (size_t)r * d.stride;
     int have = 0;          // valid entries of best[]
@@ -170,16 +173,16 @@ __global__ __launch_bounds__(THREADS, AHEAD ? 4 : THREADS == 64 ? 3 : 8) void ro
     float sum = 0.f;
     if (tid == 0) count_s[0] = 0;
     int turn = 0;
-    for (int c0 = 0; c0 < d.cols; c0 += chunk, turn ^= 1) {
+    for (int c0 = 0; c0 < d.cols; c0 += step, turn ^= 1) {
       float z[kHold];
       int t = tid;  // (columns are worked out where they are needed: hidden from the compiler, which would keep 20 of them)
       asm volatile("" : "+v"(t));
       if (AHEAD) {
         take_chunk<THREADS, VEC>(ahead, tid, z);
         const int left = d.cols - c0;
-        if (left > chunk) load_chunk<THREADS, VEC>(row + c0 + chunk, left - chunk, ahead, tid, wave);
-        else if (r + gridDim.x < d.rows) load_chunk<THREADS, VEC>(row + (size_t)gridDim.x * d.stride, d.cols, ahead, tid, wave);
-        end_chunk<THREADS, VEC>(left, t, z);
+        if (left > step) load_chunk<THREADS, VEC>(row + c0 + step, min(left - step, step), ahead, tid, wave);
+        else if (r + gridDim.x < d.rows) load_chunk<THREADS, VEC>(row + (size_t)gridDim.x * d.stride, min(d.cols, step), ahead, tid, wave);
+        end_chunk<THREADS, VEC>(min(left, step), t, z);
       } else {
         read_chunk<THREADS, VEC>(row, c0, d.cols, t, z);
       }
@@ -279,7 +282,7 @@ __global__ __launch_bounds__(THREADS, AHEAD ? 4 : THREADS == 64 ? 3 : 8) void ro
       n += have;
       if (n > kCap + have) {
         // (rare: the chunk is read again, from the cache, instead of being kept in registers for this)
-        const int end = d.cols - c0 > chunk ? c0 + chunk : d.cols;
+        const int end = d.cols - c0 > step ? c0 + step : d.cols;
         // `lo` lets too many through, `hi` too few: the keys between are distinct, so a bound that lets between K and
         // kCap through is found within 64 rounds.  A chunk of at most kCap elements is taken whole.
         key_t lo = 0, hi = ~0ull, found = end - c0 <= kCap ? 0 : hi;
