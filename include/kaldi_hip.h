@@ -494,10 +494,10 @@ int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int
  * with g = row_adapter[r].  `order` (may be NULL: the rows as they stand) is the sequence in which rows are put
  * together into tiles: give hipI32_adapter_plan's where neighbouring rows have different adapters, NULL where they lie
  * together already (utterances, single frames).  The result does not depend on it beyond rounding (a row that a broken
- * order does not list may stay unwritten).  `t` is what
- * the backward pass needs; bias may be NULL.  out and t must not overlap an input.  Rows behind N and columns
- * behind O (max_rank) are left as they are.  N <= 2^26.  Uses no library workspace: may be captured into a graph.  A row of t has
- * the same bits whoever shares its call, and with hipK_gemm_row_invariant(1) so has a row of out.
+ * order does not list may stay unwritten).  `t` is what the backward pass needs; bias may be NULL.  out and t must
+ * not overlap an input.  Rows behind N and columns behind O (max_rank) are left as they are.  N <= 2^26; I, O <= 2^30.
+ * Uses no library workspace: may be captured into a graph.  A row of t has the same bits whoever shares its call, and
+ * with hipK_gemm_row_invariant(1) so has a row of out.
  * Arithmetic: every float is taken as the sum of three bfloat16 numbers (24 bits of mantissa: exact) and a product
  * of two floats as the six largest of the nine part products, on the matrix cores with float sums; what is left out
  * is below 2^-26 of the product, less than one rounding of a float product.  An infinity or NaN in a row of `in`
@@ -532,8 +532,8 @@ int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t I, const f
  * NaN above every number: idx[r,k] = column, val[r,k] = mat[r, idx[r,k]].  K beyond the row's length fills up with
  * idx -1, val -inf.  lse[r] = log(sum_c exp(mat[r,c])) (may be NULL; -inf for a row of -inf, NaN for
  * one that holds a NaN or +inf), so that val - lse are log-posteriors.  What hipF_find_row_max_id is for one
- * maximum; it makes a teacher's outputs small enough to keep.  The outputs must not overlap mat.  Uses no library
- * workspace. */
+ * maximum; it makes a teacher's outputs small enough to keep.  The outputs must not overlap mat.  At most 2^30
+ * columns.  Uses no library workspace. */
 int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t K, int32_t *idx, int32_t ldidx, float *val,
                  int32_t ldval, float *lse);
 
@@ -548,7 +548,8 @@ int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t K, int32_t
  * [0, cols) is none, its part of the row is zero.  w = weight[r] (NULL = 1); a row of weight 0, and a row whose x are
  * all -inf, get loss 0 and a gradient of zeros whatever the row holds.  row_loss (rows floats) may be NULL if loss is;
  * loss[0] += sum of row_loss (double on the device, summed in row order; may be NULL).  T > 0, 0 <= h <= 1.
- * Sums in float over at most 1024 partial sums per row, the logarithms in double.  Uses no library workspace. */
+ * Sums in float over at most 1024 partial sums per row, the logarithms in double.  At most 2^30 columns.  Uses no library
+ * workspace. */
 int hipF_distill_eval(khStream_t s, const float *x, MatrixDim d, const int32_t *idx, int32_t ldidx, const float *val,
                       int32_t ldval, int32_t K, const int32_t *label, const float *weight, float temperature,
                       float hard_weight, float *diff, int32_t lddiff, float *row_loss, double *loss);

@@ -1026,7 +1026,7 @@ void launch_wide(hipStream_t st, const WideArgs &p, const NarrowArgs &narrow, Fi
 }
 
 // A grid counts its threads in 32 bits: 2^26 rows in windows of 16 rows and 512 threads fill half of that.
-constexpr int kMaxRows = 1 << 26, kMaxAdapters = 1 << 21;
+constexpr int kMaxRows = 1 << 26, kMaxAdapters = 1 << 21, kMaxDim = 1 << 30;
 int too_many(const char *what, int n, int most) {
   snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "%d %s: at most %d", n, what, most);
   return KH_ERR_TOO_LARGE;
@@ -1035,6 +1035,7 @@ int too_many(const char *what, int n, int most) {
 int check_adapters(const khAdapters *ad, const int32_t *row_adapter, int32_t N, int32_t I, int32_t O) {
   KH_REQUIRE(ad != nullptr && ad->num >= 0);
   if (N > kMaxRows) return too_many("rows", N, kMaxRows);
+  if (std::max(I, O) > kMaxDim) return too_many("columns", std::max(I, O), kMaxDim);  // (counted in 32 bits, a step further)
   if (ad->num == 0) return KH_OK;
   KH_REQUIRE(ad->max_rank >= 1 && ad->rows >= 0);
   if (ad->max_rank > KH_MAX_ADAPTER_RANK) {

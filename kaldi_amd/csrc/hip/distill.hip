@@ -609,12 +609,19 @@ int too_large(const char *what, int K) {
   return KH_ERR_TOO_LARGE;
 }
 
+constexpr int kMaxCols = 1 << 30;  // columns are counted in 32 bits, a chunk further than the row goes
+int too_wide(int cols) {
+  snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "%d columns: at most %d", cols, kMaxCols);
+  return KH_ERR_TOO_LARGE;
+}
+
 }  // namespace
 
 KH_EXPORT int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t K, int32_t *idx, int32_t ldidx, float *val,
                            int32_t ldval, float *lse) {
   KH_REQUIRE(kh::dim_ok(d) && K >= 1 && ldidx >= K && ldval >= K);
   if (K > KH_MAX_TOP) return too_large(__func__, K);
+  if (d.cols > kMaxCols) return too_wide(d.cols);
   KH_REQUIRE(d.rows == 0 || (idx != nullptr && val != nullptr && (d.cols == 0 || mat != nullptr)));
   KH_CHECK_INIT();
   int rc = check_device();
@@ -639,6 +646,7 @@ KH_EXPORT int hipF_distill_eval(khStream_t s, const float *x, MatrixDim d, const
                                 double *loss) {
   KH_REQUIRE(kh::dim_ok(d) && K >= 1 && ldidx >= K && ldval >= K);
   if (K > KH_MAX_TOP) return too_large(__func__, K);
+  if (d.cols > kMaxCols) return too_wide(d.cols);
   KH_REQUIRE(temperature > 0.f && temperature <= 3.402823466e38f);
   KH_REQUIRE(hard_weight >= 0.f && hard_weight <= 1.f);
   KH_REQUIRE(d.rows == 0 || (idx != nullptr && val != nullptr && (d.cols == 0 || x != nullptr)));

@@ -102,6 +102,12 @@ def test_too_many():
     assert status("hipF_adapter_forward", FORWARD, N=rows, ad=adapters(num=0)) == TOO_LARGE
     assert status("hipI32_adapter_plan", PLAN, num=2 ** 21 + 1) == TOO_LARGE
     assert b"2097153" in h.lib.hipK_error_string(TOO_LARGE)
+    wide = 2 ** 30 + 1
+    assert status("hipF_adapter_forward", FORWARD, I=wide, ldin=wide, ldw=wide, ad=adapters(lddown=wide)) == TOO_LARGE
+    assert status("hipF_adapter_backward", BACKWARD, O=wide, lde=wide, ad=adapters(ldup=wide)) == TOO_LARGE
+    assert status("hipF_row_top", TOP, d=(4, wide, wide)) == TOO_LARGE
+    assert status("hipF_distill_eval", DISTILL, d=(4, wide, wide), lddiff=wide) == TOO_LARGE
+    assert b"1073741825" in h.lib.hipK_error_string(TOO_LARGE)
     # one workgroup per adapter and 32 columns
     assert status("hipF_adapter_backward", BACKWARD, ad=adapters(num=2 ** 22)) == TOO_LARGE
     assert b"48 columns" in h.lib.hipK_error_string(TOO_LARGE)
