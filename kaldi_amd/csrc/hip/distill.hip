@@ -460,7 +460,6 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs p) {
   }
   __syncthreads();
   // the row's maximum and sums
-  const float own = m == -INFINITY ? 0.f : m;  // what this wave's exponentials are relative to
   float top = max_s[0];
 #pragma unroll
   for (int i = 1; i < waves; ++i) top = fmaxf(top, max_s[i]);
@@ -481,9 +480,11 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs p) {
 
   if (out) {
     const bool single = C <= chunk;
-    // (of a single chunk: the exponentials in the registers are relative to the wave's own maximum)
-    const float st = (BOTH ? ft : ft + f1) * exp_scaled(own - base, p.soft_scale);
-    const float s1 = BOTH ? f1 * exp_scaled(own - base, one) : 0.f;
+    // (of a single chunk: the exponentials in the registers are relative to the wave's own maximum.  A wave whose columns are
+    // all -inf has none and holds zeros: 0 - base would overflow where the row lies far below 0, and 0 * inf is NaN)
+    const float off = m == -INFINITY ? 0.f : m - base;
+    const float st = (BOTH ? ft : ft + f1) * exp_scaled(off, p.soft_scale);
+    const float s1 = BOTH ? f1 * exp_scaled(off, one) : 0.f;
     for (int c0 = 0; c0 < C; c0 += chunk) {
       if (single) {
 #pragma unroll
