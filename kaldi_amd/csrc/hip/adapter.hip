@@ -138,9 +138,9 @@ struct Stack {
 __device__ __forceinline__ void stack_rows(const Stack &st, int g, int *first, int *rank) {
   int lo = st.begin[g], hi = st.begin[g + 1];
   lo = min(max(lo, 0), st.rows);
-  hi = min(hi, st.rows);
+  hi = max(min(hi, st.rows), lo);  // (a difference of what lies inside: it cannot wrap around)
   *first = lo;
-  *rank = max(0, min(hi - lo, st.max_rank));
+  *rank = min(hi - lo, st.max_rank);
 }
 
 // Row `i` of the tile sequence: the row itself or order[i]; -1 behind the end or outside the matrix.

@@ -3,7 +3,8 @@ tolerances as test_gpu_adapters.py and test_gpu_distill.py."""
 import numpy as np
 import pytest
 
-from test_gpu_distill import check_distill, table
+from test_gpu_adapters import Case, bound, within
+from test_gpu_distill import check_distill
 
 pytestmark = pytest.mark.gpu
 f32, f64 = np.float32, np.float64
@@ -34,3 +35,32 @@ def test_distill_mask_over_all_columns_of_a_wave(hip, C, threads, pad, T, level,
         there = np.flatnonzero(~gone[r])
         idx[r], label[r] = rs.permutation(there)[:K], rs.choice(there)
     check_distill(hip, x, idx, val, label if hard else None, None, T, hard, pad=pad)
+
+
+@pytest.mark.parametrize("N", [3, 50, 600])
+def test_begins_far_below_zero_stay_inside(hip, N):
+    """An adapter that ends before it begins has no rows, however far before: the stacks' neighbours are not touched, and rows of
+    such adapters come out as rows without one.  (One that begins below zero begins at zero.)"""
+    c = Case(hip, N, 33, 40, 4, 8, "shuffled", seed=4, ragged=False, none=0.0, pad=1)
+    t = c.forward(0)[1].astype(f32)
+    plain = Case(hip, N, 33, 40, 4, 8, "shuffled", seed=4, ragged=False, none=0.0)
+    plain.ids[:] = -1
+    alone, _ = plain.run_forward(0)
+    for begin in ([1, -2 ** 31, 34, -2 ** 31, -2 ** 31 + 5], [34, -2 ** 31 + 1, 34, -5, -2 ** 31], [-2 ** 31, -2 ** 31, -2 ** 31, -1, -1]):
+        c.begin = np.array(begin, np.int32)
+        out, got_t = c.run_forward(0, True)
+        u, eo, gd, gu = c.run_backward(t)  # (the windows' surroundings are checked as they come back)
+        untouched = np.ones(len(c.down), bool)
+        for g in range(4):
+            m, lo, hi = c.ids == g, max(begin[g], 0), begin[g + 1]
+            if hi <= lo:
+                assert not got_t[m].any() and not u[m].any()
+                np.testing.assert_allclose(out[m], alone[m], rtol=0, atol=1e-4)
+                continue
+            r = slice(lo, lo + min(hi - lo, 8))  # (a range longer than the largest rank is cut there)
+            untouched[r] = False
+            x, down, up, e = c.x[m].astype(f64), c.down[r].astype(f64), c.up[r].astype(f64), c.e[m].astype(f64)
+            within(got_t[m], c.scale[g] * (x @ down.T), bound(40) * c.scale[g] * (x @ np.abs(down.T)) + 1e-37)
+            within(u[m], c.scale[g] * (e @ up.T), bound(33) * c.scale[g] * (np.abs(e) @ np.abs(up.T)) + 1e-37)
+        assert np.isnan(gd[untouched]).all() and np.isnan(gu[untouched]).all()
+        assert np.isfinite(gd[~untouched]).all() and np.isfinite(gu[~untouched]).all()
