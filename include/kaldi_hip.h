@@ -483,7 +483,8 @@ typedef struct {
 /* Groups the N rows of a bunch by adapter: order[] lists the rows of adapter 0, then of adapter 1, ..., each in
  * ascending order, then the rows without one (row_adapter[r] outside [0, num)); adapter g's are
  * order[row_begin[g] .. row_begin[g+1]-1].  order: N, row_begin: num + 1 int32 on the device.  One bunch's grouping
- * serves every layer, forward and backward.  num <= 2^21. */
+ * serves every layer, forward and backward.  N <= 2^26, num <= 2^21, N * (num + 1) <= 2^40: it reads that many ids twice
+ * (a bunch is what it is made for; 2^20 rows of 2000 adapters are 16 GB out of the caches). */
 int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int32_t num, int32_t *order,
                         int32_t *row_begin);
 

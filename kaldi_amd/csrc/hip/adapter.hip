@@ -1064,7 +1064,13 @@ KH_EXPORT int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int3
                                   int32_t *row_begin) {
   KH_REQUIRE(N >= 0 && num >= 0 && row_begin != nullptr);
   KH_REQUIRE(N == 0 || (row_adapter != nullptr && order != nullptr));
+  if (N > kMaxRows) return too_many("rows", N, kMaxRows);  // (counted in 32 bits, a workgroup's 1024 further)
   if (num > kMaxAdapters) return too_many("adapters", num, kMaxAdapters);  // (a workgroup of up to 1024 for each)
+  // every workgroup reads all ids, twice: 2^40 of them are 8 TB out of the caches, about a second
+  if (N * (num + 1ll) > 1ll << 40) {
+    snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "%d rows of %d adapters: too many together", N, num);
+    return KH_ERR_TOO_LARGE;
+  }
   KH_CHECK_INIT();
   int rc = check_device();
   if (rc != KH_OK) return rc;
