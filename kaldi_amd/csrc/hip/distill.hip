@@ -556,11 +556,11 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs p) {
   }
 }
 
-// loss[0] += the rows' losses, in a fixed order
+// loss[0] += the rows' losses, in a fixed order: thread t adds rows t, t + 256, ..., then the threads' sums in a tree
 __global__ __launch_bounds__(256) void sum_rows_kernel(const float *row_loss, int rows, double *loss) {
   __shared__ double sd[4];
   double t = 0.0;
-  for (int i = threadIdx.x; i < rows; i += 256) t += (double)row_loss[i];
+  for (unsigned i = threadIdx.x; i < (unsigned)rows; i += 256) t += (double)row_loss[i];  // (past 2^31 an int would wrap around)
   t = kh::wave_sum_d(t);
   if ((threadIdx.x & 63) == 0) sd[threadIdx.x >> 6] = t;
   __syncthreads();

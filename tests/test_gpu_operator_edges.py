@@ -64,3 +64,19 @@ def test_begins_far_below_zero_stay_inside(hip, N):
             within(u[m], c.scale[g] * (e @ up.T), bound(33) * c.scale[g] * (np.abs(e) @ np.abs(up.T)) + 1e-37)
         assert np.isnan(gd[untouched]).all() and np.isnan(gu[untouched]).all()
         assert np.isfinite(gd[~untouched]).all() and np.isfinite(gu[~untouched]).all()
+
+
+def test_distill_loss_over_almost_2_to_31_rows(hip):
+    """Rows are counted past where 32 bits with a sign end: two equal logits everywhere, so every row's loss is the float next to
+    log 2.  Sums in double of fewer than 2^24 addends per thread are good to 2^24 * 2^-53 = 2^-29 of themselves."""
+    R = 2 ** 31 - 1
+    x = hip.DevMatrix(R, 2, f32, False)
+    label, row_loss = hip.DevMatrix(1, R, np.int32, False), hip.DevMatrix(1, R, f32, False)
+    loss = hip.DevMatrix(1, 1, f64, False)
+    # (the teacher's table is not looked at where only hard labels count)
+    hip.call("hipF_distill_eval", None, x.ptr, hip.MatrixDim(R, 2, 2), label.ptr, 1, x.ptr, 1, 1, label.ptr, None, 1.0, 1.0, None, 0,
+             row_loss.ptr, loss.ptr)
+    want = R * float(f32(np.log(2.0)))
+    assert abs(loss.numpy()[0, 0] - want) <= 2.0 ** -29 * want
+    for m in (x, label, row_loss):
+        m.free()
