@@ -5,6 +5,7 @@
 // bunch.
 #ifndef KALDI_AMD_NNET_NNET_ADAPTERS_H_
 #define KALDI_AMD_NNET_NNET_ADAPTERS_H_
+#include <limits>
 #include <vector>
 
 #include "base/io-funcs.h"
@@ -54,20 +55,24 @@ class Adapters {
  public:
   Adapters() {}
 
-  /// Adapters of the given ranks (each 0 .. KH_MAX_ADAPTER_RANK) for a layer input_dim -> output_dim, all weights 0.
+  /// Adapters of the given ranks (each 0 .. KH_MAX_ADAPTER_RANK) for a layer input_dim -> output_dim, all weights 0.  What is
+  /// refused leaves the adapters as they were; where the device has no memory for the new ones, there are none afterwards.
   void Init(int32 input_dim, int32 output_dim, const std::vector<int32> &ranks, const std::vector<BaseFloat> &scale) {
     KALDI_ASSERT(input_dim > 0 && output_dim > 0 && ranks.size() == scale.size());
-    input_dim_ = input_dim;
-    output_dim_ = output_dim;
-    ranks_ = ranks;
     std::vector<int32> begin(1, 0);
-    max_rank_ = 1;
+    int32 max_rank = 1;
+    int64 rows = 0;
     for (size_t g = 0; g < ranks.size(); ++g) {
       if (ranks[g] < 0 || ranks[g] > KH_MAX_ADAPTER_RANK)
         KALDI_ERR << "Adapter " << g << " of rank " << ranks[g] << ": 0 to " << KH_MAX_ADAPTER_RANK << " are supported";
-      begin.push_back(begin.back() + ranks[g]);
-      if (ranks[g] > max_rank_) max_rank_ = ranks[g];
+      rows += ranks[g];
+      if (rows > std::numeric_limits<int32>::max()) KALDI_ERR << "Adapters of more than 2^31 - 1 rows together";
+      begin.push_back(static_cast<int32>(rows));
+      if (ranks[g] > max_rank) max_rank = ranks[g];
     }
+    // none, until everything is there: the number of adapters is what the kernels read `begin` and `scale` by
+    ranks_.clear();
+    input_dim_ = output_dim_ = 0;
     begin_.CopyFromVec(begin);
     Vector<BaseFloat> s(scale.size());
     for (size_t g = 0; g < scale.size(); ++g) s(g) = scale[g];
@@ -76,6 +81,10 @@ class Adapters {
     up_.Resize(begin.back(), output_dim);
     down_.SetZero();
     up_.SetZero();
+    max_rank_ = max_rank;
+    input_dim_ = input_dim;
+    output_dim_ = output_dim;
+    ranks_ = ranks;
   }
 
   int32 NumAdapters() const { return static_cast<int32>(ranks_.size()); }

@@ -1,0 +1,114 @@
+// The adapter classes where a call goes wrong or has nothing to do; tests/test_adapter_classes.py and
+// tests/test_gpu_adapter_classes.py look at what is printed.
+//
+// usage: adapter_edges_walk read <adapters-file>    a file that is refused, into empty adapters (no device is needed)
+//        adapter_edges_walk reread <adapters-file>  the same into adapters that are in use
+#include <cstdio>
+#include <fstream>
+#include <iostream>
+#include <string>
+#include <vector>
+
+#include "base/kaldi-common.h"
+#include "cudamatrix/cu-math.h"
+#include "nnet/nnet-adapters.h"
+#include "nnet/nnet-biasedlinearity.h"
+
+using namespace kaldi;
+
+namespace {
+
+// true if the file was refused
+bool Refused(Adapters *adapters, const char *file) {
+  std::ifstream is(file, std::ios::binary);
+  if (!is) {
+    fprintf(stderr, "cannot read %s\n", file);
+    exit(1);
+  }
+  try {
+    adapters->Read(is, false);
+  } catch (const std::exception &e) {
+    std::cerr << e.what();
+    return true;
+  }
+  return false;
+}
+
+void Fill(Matrix<BaseFloat> *m, float scale) {
+  for (int32 r = 0; r < m->NumRows(); ++r)
+    for (int32 c = 0; c < m->NumCols(); ++c) (*m)(r, c) = scale * static_cast<float>((7 * r + 3 * c) % 11 - 5);
+}
+
+// a layer, the adapters of some speakers and a bunch of rows
+struct Bench {
+  static const int32 kRows = 37, kIn = 12, kOut = 9;
+  BiasedLinearity layer;
+  CuMatrix<BaseFloat> x, err;
+  Adapters adapters;
+  AdapterRows who;
+  int32 num;
+  Bench() : layer(kIn, kOut, NULL), num(3) {
+    Matrix<BaseFloat> w(kOut, kIn), in(kRows, kIn), e(kRows, kOut), down(6, kIn), up(6, kOut);
+    Vector<BaseFloat> b(kOut);
+    for (int32 i = 0; i < kOut; ++i) b(i) = 0.1f * i;
+    Fill(&w, 0.05f);
+    Fill(&in, 0.2f);
+    Fill(&e, 0.1f);
+    Fill(&down, 0.1f);
+    Fill(&up, 0.1f);
+    layer.SetLinearityWeight(w, false);
+    layer.SetBiasWeight(b);
+    x.CopyFromMat(in);
+    err.CopyFromMat(e);
+    adapters.Init(kIn, kOut, std::vector<int32>({1, 2, 3}), std::vector<BaseFloat>({1.0f, 0.5f, 2.0f}));
+    adapters.SetDown(down);
+    adapters.SetUp(up);
+    std::vector<int32> ids;
+    for (int32 r = 0; r < kRows; ++r) ids.push_back(r % (num + 1) - 1);
+    who.Set(ids, num);
+  }
+};
+
+std::vector<float> Values(const CuMatrix<BaseFloat> &m) {
+  Matrix<BaseFloat> h;
+  m.CopyToMat(&h);
+  std::vector<float> v;
+  for (int32 r = 0; r < h.NumRows(); ++r)
+    for (int32 c = 0; c < h.NumCols(); ++c) v.push_back(h(r, c));
+  return v;
+}
+
+int Read(const char *file) {
+  Adapters a;
+  const bool refused = Refused(&a, file);
+  printf("refused %d adapters %d %d -> %d\n", refused, a.NumAdapters(), a.InputDim(), a.OutputDim());
+  return 0;
+}
+
+int Reread(const char *file) {
+  Bench s;
+  CuMatrix<BaseFloat> before, after;
+  s.adapters.Propagate(&s.layer, s.x, s.who, KH_ACT_SIGMOID, &before);
+  const bool refused = Refused(&s.adapters, file);
+  printf("refused %d adapters %d %d -> %d\n", refused, s.adapters.NumAdapters(), s.adapters.InputDim(), s.adapters.OutputDim());
+  fflush(stdout);
+  s.adapters.Propagate(&s.layer, s.x, s.who, KH_ACT_SIGMOID, &after);
+  printf("same %d\n", Values(before) == Values(after));
+  return 0;
+}
+
+}  // namespace
+
+int main(int argc, char **argv) {
+  const std::string what = argc > 1 ? argv[1] : "";
+  try {
+    if (what == "read" && argc == 3) return Read(argv[2]);
+    CuDevice::Instantiate().SelectGpuId(-1);
+    if (what == "reread" && argc == 3) return Reread(argv[2]);
+    fprintf(stderr, "usage: adapter_edges_walk read|reread <adapters-file>\n");
+    return 1;
+  } catch (const std::exception &e) {
+    std::cerr << e.what();
+    return 255;
+  }
+}

@@ -1,0 +1,17 @@
+"""The adapter classes where a call goes wrong or has nothing to do (tests/fuzz/adapter_edges_walk.cc)."""
+import subprocess
+
+import pytest
+
+from test_adapter_classes import BAD, WALK
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("what", sorted(BAD))
+def test_adapters_in_use_survive_a_refused_file(tmp_path, what):
+    f = tmp_path / "adapters"
+    f.write_text(BAD[what])
+    r = subprocess.run([WALK, "reread", str(f)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
+    assert r.stdout.split("\n")[:2] == ["refused 1 adapters 3 12 -> 9", "same 1"]
