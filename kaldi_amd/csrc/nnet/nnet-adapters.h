@@ -73,6 +73,10 @@ class Adapters {
     // none, until everything is there: the number of adapters is what the kernels read `begin` and `scale` by
     ranks_.clear();
     input_dim_ = output_dim_ = 0;
+    t_.Resize(0, 0);  // (what a forward and a backward pass left is of the adapters before)
+    u_.Resize(0, 0);
+    down_grad_.Resize(0, 0);
+    up_grad_.Resize(0, 0);
     begin_.CopyFromVec(begin);
     Vector<BaseFloat> s(scale.size());
     for (size_t g = 0; g < scale.size(); ++g) s(g) = scale[g];
@@ -125,8 +129,9 @@ class Adapters {
                      const AdapterRows &rows, const CuMatrix<BaseFloat> *y, CuMatrix<BaseFloat> *out_err) {
     CuProfileScope p("Adapters::Backpropagate");
     Check(layer, in, rows);
-    KALDI_ASSERT(in_err.NumRows() == in.NumRows() && in_err.NumCols() == output_dim_ && t_.NumRows() == in.NumRows() &&
-                 t_.NumCols() == max_rank_);
+    KALDI_ASSERT(in_err.NumRows() == in.NumRows() && in_err.NumCols() == output_dim_);
+    if (t_.NumRows() != in.NumRows() || (in.NumRows() > 0 && t_.NumCols() != max_rank_))
+      KALDI_ERR << "Adapters: no forward pass of these " << in.NumRows() << " rows";
     KALDI_ASSERT(y == NULL || (y->NumRows() == in.NumRows() && y->NumCols() == input_dim_));
     if (out_err && (out_err->NumRows() != in.NumRows() || out_err->NumCols() != input_dim_))
       out_err->Resize(in.NumRows(), input_dim_);
@@ -142,10 +147,11 @@ class Adapters {
         down_grad_.Data(), down_grad_.Stride(), up_grad_.Data(), up_grad_.Stride()));
   }
 
-  /// a step against the gradients
+  /// a step against the gradients of the last Backpropagate; refused where Init or Read came behind it
   void Update(BaseFloat learn_rate) {
     CuProfileScope p("Adapters::Update");
-    KALDI_ASSERT(down_grad_.NumRows() == down_.NumRows() && up_grad_.NumRows() == up_.NumRows());
+    if (down_grad_.NumRows() != down_.NumRows() || up_grad_.NumRows() != up_.NumRows())
+      KALDI_ERR << "Adapters: no gradients of these adapters";
     down_.AddMat(-learn_rate, down_grad_);
     up_.AddMat(-learn_rate, up_grad_);
   }

@@ -3,6 +3,7 @@
 //
 // usage: adapter_edges_walk read <adapters-file>    a file that is refused, into empty adapters (no device is needed)
 //        adapter_edges_walk reread <adapters-file>  the same into adapters that are in use
+//        adapter_edges_walk stale <adapters-file>   a good file into adapters that hold a forward pass and gradients
 #include <cstdio>
 #include <fstream>
 #include <iostream>
@@ -97,6 +98,45 @@ int Reread(const char *file) {
   return 0;
 }
 
+template <class F>
+bool Throws(F f) {
+  try {
+    f();
+  } catch (const std::exception &e) {
+    std::cerr << e.what();
+    return true;
+  }
+  return false;
+}
+
+int Stale(const char *file) {
+  Bench s;
+  CuMatrix<BaseFloat> out;
+  s.adapters.Propagate(&s.layer, s.x, s.who, KH_ACT_SIGMOID, &out);
+  s.adapters.Backpropagate(&s.layer, s.x, s.err, s.who, NULL, NULL);
+  {
+    std::ofstream os(file, std::ios::binary);
+    s.adapters.Write(os, true);
+  }
+  std::ifstream is(file, std::ios::binary), is2(file, std::ios::binary);
+  Adapters fresh;
+  fresh.Read(is, true);
+  s.adapters.Read(is2, true);
+  const std::vector<float> down = Values(s.adapters.Down()), up = Values(s.adapters.Up());
+  printf("update refused %d\n", Throws([&] { s.adapters.Update(0.1f); }));
+  printf("weights same %d\n", down == Values(s.adapters.Down()) && up == Values(s.adapters.Up()));
+  printf("backpropagate refused %d\n", Throws([&] { s.adapters.Backpropagate(&s.layer, s.x, s.err, s.who, NULL, NULL); }));
+  Adapters *both[2] = {&s.adapters, &fresh};
+  for (int i = 0; i < 2; ++i) {
+    both[i]->Propagate(&s.layer, s.x, s.who, KH_ACT_SIGMOID, &out);
+    both[i]->Backpropagate(&s.layer, s.x, s.err, s.who, NULL, NULL);
+    both[i]->Update(0.1f);
+  }
+  printf("as fresh ones %d\n", Values(s.adapters.Down()) == Values(fresh.Down()) && Values(s.adapters.Up()) == Values(fresh.Up()) &&
+                                    Values(fresh.Up()) != up);
+  return 0;
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -105,7 +145,8 @@ int main(int argc, char **argv) {
     if (what == "read" && argc == 3) return Read(argv[2]);
     CuDevice::Instantiate().SelectGpuId(-1);
     if (what == "reread" && argc == 3) return Reread(argv[2]);
-    fprintf(stderr, "usage: adapter_edges_walk read|reread <adapters-file>\n");
+    if (what == "stale" && argc == 3) return Stale(argv[2]);
+    fprintf(stderr, "usage: adapter_edges_walk read|reread|stale <adapters-file>\n");
     return 1;
   } catch (const std::exception &e) {
     std::cerr << e.what();

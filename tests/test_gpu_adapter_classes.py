@@ -15,3 +15,10 @@ def test_adapters_in_use_survive_a_refused_file(tmp_path, what):
     r = subprocess.run([WALK, "reread", str(f)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stderr
     assert r.stdout.split("\n")[:2] == ["refused 1 adapters 3 12 -> 9", "same 1"]
+
+
+def test_adapters_of_a_file_have_no_gradients_yet(tmp_path):
+    """What the adapters before the file left behind (gradients, the narrow products of a forward pass) is not theirs."""
+    r = subprocess.run([WALK, "stale", str(tmp_path / "adapters")], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
+    assert r.stdout.split("\n")[:4] == ["update refused 1", "weights same 1", "backpropagate refused 1", "as fresh ones 1"]
