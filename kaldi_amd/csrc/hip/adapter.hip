@@ -1044,7 +1044,7 @@ int check_adapters(const khAdapters *ad, const int32_t *row_adapter, int32_t N, 
              KH_MAX_ADAPTER_RANK);
     return KH_ERR_TOO_LARGE;
   }
-  KH_REQUIRE(ad->begin != nullptr && row_adapter != nullptr);
+  KH_REQUIRE(ad->begin != nullptr && (N == 0 || row_adapter != nullptr));
   KH_REQUIRE(ad->rows == 0 || (ad->down != nullptr && ad->up != nullptr));
   KH_REQUIRE(ad->lddown >= I && ad->ldup >= O);
   return KH_OK;

@@ -129,10 +129,10 @@ class Adapters {
                      const AdapterRows &rows, const CuMatrix<BaseFloat> *y, CuMatrix<BaseFloat> *out_err) {
     CuProfileScope p("Adapters::Backpropagate");
     Check(layer, in, rows);
-    KALDI_ASSERT(in_err.NumRows() == in.NumRows() && in_err.NumCols() == output_dim_);
+    KALDI_ASSERT(in_err.NumRows() == in.NumRows() && (in.NumRows() == 0 || in_err.NumCols() == output_dim_));
     if (t_.NumRows() != in.NumRows() || (in.NumRows() > 0 && t_.NumCols() != max_rank_))
       KALDI_ERR << "Adapters: no forward pass of these " << in.NumRows() << " rows";
-    KALDI_ASSERT(y == NULL || (y->NumRows() == in.NumRows() && y->NumCols() == input_dim_));
+    KALDI_ASSERT(y == NULL || (y->NumRows() == in.NumRows() && (in.NumRows() == 0 || y->NumCols() == input_dim_)));
     if (out_err && (out_err->NumRows() != in.NumRows() || out_err->NumCols() != input_dim_))
       out_err->Resize(in.NumRows(), input_dim_);
     u_.Resize(in.NumRows(), max_rank_);
@@ -204,7 +204,9 @@ class Adapters {
     return ad;
   }
   void Check(BiasedLinearity *layer, const CuMatrix<BaseFloat> &in, const AdapterRows &rows) const {
-    if (layer->InputDim() != input_dim_ || layer->OutputDim() != output_dim_ || in.NumCols() != input_dim_)
+    // (a matrix without rows has no columns either)
+    if (layer->InputDim() != input_dim_ || layer->OutputDim() != output_dim_ ||
+        (in.NumRows() > 0 && in.NumCols() != input_dim_))
       KALDI_ERR << "Nonmatching dims, adapters:" << input_dim_ << "->" << output_dim_ << " layer:" << layer->InputDim() << "->"
                 << layer->OutputDim() << " data:" << in.NumCols();
     KALDI_ASSERT(rows.NumRows() == in.NumRows() && rows.NumAdapters() == NumAdapters());

@@ -4,6 +4,7 @@
 // usage: adapter_edges_walk read <adapters-file>    a file that is refused, into empty adapters (no device is needed)
 //        adapter_edges_walk reread <adapters-file>  the same into adapters that are in use
 //        adapter_edges_walk stale <adapters-file>   a good file into adapters that hold a forward pass and gradients
+//        adapter_edges_walk empty                   a bunch without rows
 #include <cstdio>
 #include <fstream>
 #include <iostream>
@@ -137,6 +138,32 @@ int Stale(const char *file) {
   return 0;
 }
 
+bool AllZero(const CuMatrix<BaseFloat> &m, int32 rows, int32 cols) {
+  const std::vector<float> v = Values(m);
+  for (size_t i = 0; i < v.size(); ++i)
+    if (v[i] != 0.0f) return false;
+  return m.NumRows() == rows && m.NumCols() == cols;
+}
+
+int Empty() {
+  Bench s;
+  CuMatrix<BaseFloat> out, below, nothing;
+  AdapterRows none;
+  none.Set(std::vector<int32>(), s.num);
+  for (int turn = 0; turn < 2; ++turn) {  // behind nothing, and behind a bunch with rows
+    s.adapters.Propagate(&s.layer, nothing, none, KH_ACT_SIGMOID, &out);
+    s.adapters.Backpropagate(&s.layer, nothing, nothing, none, &nothing, &below);
+    printf("out %d below %d gradients zero %d\n", out.NumRows(), below.NumRows(),
+           AllZero(s.adapters.DownGradient(), 6, s.kIn) && AllZero(s.adapters.UpGradient(), 6, s.kOut));
+    s.adapters.Update(1.0f);
+    s.adapters.Propagate(&s.layer, s.x, s.who, KH_ACT_SIGMOID, &out);
+    s.adapters.Backpropagate(&s.layer, s.x, s.err, s.who, &s.x, &below);
+    printf("out %d below %d gradients zero %d\n", out.NumRows(), below.NumRows(),
+           AllZero(s.adapters.DownGradient(), 6, s.kIn) && AllZero(s.adapters.UpGradient(), 6, s.kOut));
+  }
+  return 0;
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -145,8 +172,9 @@ int main(int argc, char **argv) {
     if (what == "read" && argc == 3) return Read(argv[2]);
     CuDevice::Instantiate().SelectGpuId(-1);
     if (what == "reread" && argc == 3) return Reread(argv[2]);
+    if (what == "empty" && argc == 2) return Empty();
     if (what == "stale" && argc == 3) return Stale(argv[2]);
-    fprintf(stderr, "usage: adapter_edges_walk read|reread|stale <adapters-file>\n");
+    fprintf(stderr, "usage: adapter_edges_walk read|reread|stale <adapters-file> | empty\n");
     return 1;
   } catch (const std::exception &e) {
     std::cerr << e.what();

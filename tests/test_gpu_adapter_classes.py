@@ -22,3 +22,10 @@ def test_adapters_of_a_file_have_no_gradients_yet(tmp_path):
     r = subprocess.run([WALK, "stale", str(tmp_path / "adapters")], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stderr
     assert r.stdout.split("\n")[:4] == ["update refused 1", "weights same 1", "backpropagate refused 1", "as fresh ones 1"]
+
+
+def test_a_bunch_without_rows(tmp_path):
+    """... has outputs without rows and gradients of zeros, in front of a bunch with rows and behind one."""
+    r = subprocess.run([WALK, "empty"], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
+    assert r.stdout.split("\n")[:4] == ["out 0 below 0 gradients zero 1", "out 37 below 37 gradients zero 0"] * 2
