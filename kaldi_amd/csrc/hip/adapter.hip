@@ -1071,8 +1071,11 @@ KH_EXPORT int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int3
     snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "%d rows of %d adapters: too many together", N, num);
     return KH_ERR_TOO_LARGE;
   }
+  int rc = kh::check_apart(__func__, {{"order", order, 1, N, N}, {"row_begin", row_begin, 1, num + 1ll, num + 1ll}},
+                           {{"row_adapter", row_adapter, 1, N, N}});
+  if (rc != KH_OK) return rc;
   KH_CHECK_INIT();
-  int rc = check_device();
+  rc = check_device();
   if (rc != KH_OK) return rc;
   const int threads = N <= 256 ? 256 : 1024;
   plan_kernel<<<(unsigned)num + 1u, threads, 0, kh::pick(s)>>>(row_adapter, N, num, order, row_begin);
@@ -1088,8 +1091,15 @@ KH_EXPORT int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, 
   int rc = check_adapters(ad, row_adapter, N, I, O);
   if (rc != KH_OK) return rc;
   KH_REQUIRE(N == 0 || (ldin >= I && ldw >= I && ldout >= O));
-  KH_REQUIRE(ad->num == 0 || N == 0 || (t != nullptr && t != out && ldt >= ad->max_rank));
-  KH_REQUIRE(N == 0 || O == 0 || (out != nullptr && out != in && (I == 0 || (in != nullptr && W != nullptr))));
+  KH_REQUIRE(ad->num == 0 || N == 0 || (t != nullptr && ldt >= ad->max_rank));
+  KH_REQUIRE(N == 0 || O == 0 || (out != nullptr && (I == 0 || (in != nullptr && W != nullptr))));
+  const int num = ad->num, stack_rows = num > 0 ? ad->rows : 0;
+  rc = kh::check_apart(__func__, {{"out", out, N, O, ldout}, {"t", num > 0 ? t : nullptr, N, ad->max_rank, ldt}},
+                       {{"in", in, N, I, ldin}, {"W", W, O, I, ldw}, {"bias", bias, 1, O, O},
+                        {"down", ad->down, stack_rows, I, ad->lddown}, {"up", ad->up, stack_rows, O, ad->ldup},
+                        {"begin", ad->begin, num > 0, num + 1ll, num + 1ll}, {"scale", ad->scale, num > 0, num, num},
+                        {"row_adapter", row_adapter, num > 0, N, N}, {"order", order, 1, N, N}});
+  if (rc != KH_OK) return rc;
   KH_CHECK_INIT();
   rc = check_device();
   if (rc != KH_OK) return rc;
@@ -1128,9 +1138,8 @@ KH_EXPORT int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t 
   const int cols = grads && ad->rows > 0 ? std::max(gdown != nullptr ? I : 0, gup != nullptr ? O : 0) : 0;
   const int col_tiles = (cols + 31) / 32;
   KH_REQUIRE(N == 0 || O == 0 || (e != nullptr && lde >= O));
-  KH_REQUIRE(eout == nullptr || (W != nullptr && ldw >= I && ldeout >= I && eout != e && eout != in));
-  KH_REQUIRE(eout == nullptr || (eout != u && eout != y && (y == nullptr || ldy >= I)));
-  KH_REQUIRE(ad->num == 0 || N == 0 || (u != nullptr && ldu >= ad->max_rank && u != t));
+  KH_REQUIRE(eout == nullptr || (W != nullptr && ldw >= I && ldeout >= I && (y == nullptr || ldy >= I)));
+  KH_REQUIRE(ad->num == 0 || N == 0 || (u != nullptr && ldu >= ad->max_rank));
   KH_REQUIRE(!grads || (row_begin != nullptr && (N == 0 || order != nullptr)));
   KH_REQUIRE(gdown == nullptr || (ldgdown >= I && (N == 0 || (in != nullptr && ldin >= I))));
   KH_REQUIRE(gup == nullptr || (ldgup >= O && (N == 0 || (t != nullptr && ldt >= ad->max_rank))));
@@ -1138,6 +1147,18 @@ KH_EXPORT int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t 
     snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "gradients of %d adapters of %d columns: too many", ad->num, cols);
     return KH_ERR_TOO_LARGE;
   }
+  // (what a call does not read or write may be anywhere)
+  const int num = ad->num, stack_rows = num > 0 ? ad->rows : 0, grad_rows = grads ? stack_rows : 0;
+  rc = kh::check_apart(__func__,
+                       {{"u", num > 0 ? u : nullptr, N, ad->max_rank, ldu}, {"eout", eout, N, I, ldeout},
+                        {"gdown", gdown, grad_rows, I, ldgdown}, {"gup", gup, grad_rows, O, ldgup}},
+                       {{"e", e, N, O, lde}, {"in", gdown ? in : nullptr, N, I, ldin}, {"W", eout ? W : nullptr, O, I, ldw},
+                        {"y", eout ? y : nullptr, N, I, ldy}, {"t", gup ? t : nullptr, N, ad->max_rank, ldt},
+                        {"down", ad->down, eout ? stack_rows : 0, I, ad->lddown}, {"up", ad->up, stack_rows, O, ad->ldup},
+                        {"begin", ad->begin, num > 0, num + 1ll, num + 1ll}, {"scale", ad->scale, num > 0, num, num},
+                        {"row_adapter", row_adapter, num > 0, N, N}, {"order", order, 1, N, N},
+                        {"row_begin", row_begin, grads, num + 1ll, num + 1ll}});
+  if (rc != KH_OK) return rc;
   KH_CHECK_INIT();
   rc = check_device();
   if (rc != KH_OK) return rc;

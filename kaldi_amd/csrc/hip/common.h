@@ -6,7 +6,10 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <initializer_list>
+
 #include "kaldi_hip.h"
+#include "overlap.h"
 
 #define KH_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -68,6 +71,21 @@ inline bool aligned16(const void *p) { return (((uintptr_t)p) & 15u) == 0; }
 
 // d describes a matrix that a kernel may index: reject anything a kernel would fault on.
 inline bool dim_ok(MatrixDim d) { return d.rows >= 0 && d.cols >= 0 && d.stride >= d.cols; }
+
+// Outputs share no element with each other or with an input: what a kernel reads, another part of it may have written.
+inline int check_apart(const char *func, std::initializer_list<Area> outputs, std::initializer_list<Area> inputs) {
+  for (const Area *o = outputs.begin(); o != outputs.end(); ++o) {
+    const Area *hit = nullptr;
+    for (const Area *p = outputs.begin(); p != o; ++p)
+      if (overlap(*o, *p)) hit = p;
+    for (const Area &p : inputs)
+      if (overlap(*o, p)) hit = &p;
+    if (!hit) continue;
+    snprintf(ctx().last_msg, sizeof(ctx().last_msg), "%s: %s and %s overlap", func, o->name, hit->name);
+    return KH_ERR_INVALID_ARG;
+  }
+  return KH_OK;
+}
 
 }  // namespace kh
 

@@ -624,8 +624,11 @@ KH_EXPORT int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t 
   if (K > KH_MAX_TOP) return too_large(__func__, K);
   if (d.cols > kMaxCols) return too_wide(d.cols);
   KH_REQUIRE(d.rows == 0 || (idx != nullptr && val != nullptr && (d.cols == 0 || mat != nullptr)));
+  int rc = kh::check_apart(__func__, {{"idx", idx, d.rows, K, ldidx}, {"val", val, d.rows, K, ldval}, {"lse", lse, 1, d.rows, d.rows}},
+                           {{"mat", mat, d.rows, d.cols, d.stride}});
+  if (rc != KH_OK) return rc;
   KH_CHECK_INIT();
-  int rc = check_device();
+  rc = check_device();
   if (rc != KH_OK) return rc;
   if (d.rows == 0) return KH_OK;
   hipStream_t st = kh::pick(s);
@@ -655,8 +658,17 @@ KH_EXPORT int hipF_distill_eval(khStream_t s, const float *x, MatrixDim d, const
   KH_REQUIRE(diff == nullptr || lddiff >= d.cols);
   KH_REQUIRE(diff != x || lddiff == d.stride);
   KH_REQUIRE(loss == nullptr || d.rows == 0 || row_loss != nullptr);
+  // (diff may be x itself; the table is not read where only hard labels count, labels not where they do not)
+  const int table_rows = hard_weight < 1.f ? d.rows : 0;
+  int rc = kh::check_apart(__func__,
+                           {{"diff", diff, d.rows, d.cols, lddiff}, {"row_loss", row_loss, 1, d.rows, d.rows}, {"loss", loss, d.rows > 0, 2, 2}},
+                           {{"x", diff == x ? nullptr : x, d.rows, d.cols, d.stride}, {"idx", idx, table_rows, K, ldidx},
+                            {"val", val, table_rows, K, ldval}, {"label", label, hard_weight > 0.f, d.rows, d.rows},
+                            {"weight", weight, 1, d.rows, d.rows}});
+  // (with diff in the place of x, what overlaps x overlaps diff)
+  if (rc != KH_OK) return rc;
   KH_CHECK_INIT();
-  int rc = check_device();
+  rc = check_device();
   if (rc != KH_OK) return rc;
   if (d.rows == 0) return KH_OK;
   hipStream_t st = kh::pick(s);

@@ -1,5 +1,7 @@
 """The adapter, top-logit and distillation entry points at the ends of what their interface allows, against the same oracles and
 tolerances as test_gpu_adapters.py and test_gpu_distill.py."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -80,3 +82,32 @@ def test_distill_loss_over_almost_2_to_31_rows(hip):
     assert abs(loss.numpy()[0, 0] - want) <= 2.0 ** -29 * want
     for m in (x, label, row_loss):
         m.free()
+
+
+def side_by_side(h, rows, *cols):
+    """A buffer of NaN, and where matrices of these columns begin that lie next to each other in its rows."""
+    m = h.DevMatrix.from_numpy(np.full((rows, sum(cols) + 3), np.nan, f32), False)
+    at = np.concatenate([[1], 1 + np.cumsum(cols)])[:-1]
+    return m, [ctypes.c_void_p(m.ptr.value + 4 * int(a)) for a in at], [slice(a, a + c) for a, c in zip(at, cols)]
+
+
+@pytest.mark.parametrize("N", [1, 40, 700])
+def test_outputs_side_by_side_in_one_matrix(hip, N):
+    """Matrices that share rows of a larger one, and no element, are apart: the same bits as with each on its own."""
+    h = hip
+    c = Case(h, N, 50, 70, 5, 9, "shuffled", seed=N, pad=1)
+    out, t = c.run_forward(1, True)
+    grads = c.run_backward(t)
+    ad = c.adapters()
+    x, W, e = c.put("x", c.x), c.put("W", c.W), c.put("e", c.e)
+    ids, order, begin = c.vec(c.ids), c.vec(c.order), c.vec(c.row_begin)
+    m, (pt, pout, pu, peout), (st, sout, su, seout) = side_by_side(h, N, 9, 50, 9, 70)
+    h.call("hipF_adapter_forward", None, 1, N, 50, 70, *x, *W, c.vec(c.bias), ctypes.byref(ad), ids, order, pt, m.stride, pout, m.stride)
+    g, (pgd, pgu), (sgd, sgu) = side_by_side(h, len(c.down), 70, 50)
+    h.call("hipF_adapter_backward", None, N, 50, 70, *e, *x, *W, ctypes.byref(ad), ids, order, begin, pt, m.stride, pu, m.stride, *x,
+           peout, m.stride, pgd, g.stride, pgu, g.stride)
+    got, gg = m.numpy(), g.numpy()
+    for a, b in ((got[:, sout], out), (got[:, st], t), (got[:, su], grads[0]), (got[:, seout], grads[1]), (gg[:, sgd], grads[2]),
+                 (gg[:, sgu], grads[3])):
+        assert np.array_equal(a, b, equal_nan=True)
+    assert np.isnan(got[:, [0, -2, -1]]).all() and np.isnan(gg[:, [0, -2, -1]]).all()
