@@ -88,6 +88,7 @@ template <typename Real>
 void RowTop(const CuMatrix<Real> &mat, int32 k, CuStlVector<int32> *id, CuMatrix<Real> *val, CuVector<Real> *lse) {
   CuProfileScope p(__func__);
   KALDI_ASSERT(k >= 1);
+  if (val == &mat) KALDI_ERR << "RowTop: the values in the place of the matrix";  // (it would be resized, and with that lost)
   id->Resize(static_cast<size_t>(mat.NumRows()) * k);
   val->Resize(mat.NumRows(), k);
   if (lse) lse->Resize(mat.NumRows());

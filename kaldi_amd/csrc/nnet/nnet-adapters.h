@@ -114,6 +114,7 @@ class Adapters {
                  CuMatrix<BaseFloat> *out) {
     CuProfileScope p("Adapters::Propagate");
     Check(layer, in, rows);
+    if (out == &in) KALDI_ERR << "Adapters: the output is the input";  // (it would be resized, and with that lost)
     if (out->NumRows() != in.NumRows() || out->NumCols() != output_dim_) out->Resize(in.NumRows(), output_dim_);
     t_.Resize(in.NumRows(), max_rank_);
     const khAdapters ad = Describe();
@@ -133,6 +134,8 @@ class Adapters {
     if (t_.NumRows() != in.NumRows() || (in.NumRows() > 0 && t_.NumCols() != max_rank_))
       KALDI_ERR << "Adapters: no forward pass of these " << in.NumRows() << " rows";
     KALDI_ASSERT(y == NULL || (y->NumRows() == in.NumRows() && (in.NumRows() == 0 || y->NumCols() == input_dim_)));
+    if (out_err && (out_err == &in || out_err == &in_err || out_err == y))
+      KALDI_ERR << "Adapters: the error of the layer below is an input";
     if (out_err && (out_err->NumRows() != in.NumRows() || out_err->NumCols() != input_dim_))
       out_err->Resize(in.NumRows(), input_dim_);
     u_.Resize(in.NumRows(), max_rank_);

@@ -128,6 +128,7 @@ void Distill::Eval(const CuMatrix<BaseFloat> &net_out, const CuStlVector<int32> 
   KALDI_ASSERT(val.NumRows() == n && id.Dim() == static_cast<size_t>(n) * k);
   KALDI_ASSERT(label == NULL || static_cast<int32>(label->Dim()) == n);
   KALDI_ASSERT(weight == NULL || static_cast<int32>(weight->Dim()) == n);
+  if (diff == &val) KALDI_ERR << "Distill: the gradient in the place of the teacher's logits";
   if (diff && diff != &net_out) diff->Resize(n, net_out.NumCols());
   row_loss_.Resize(n);
   if (n == 0) return;

@@ -5,6 +5,7 @@
 //        adapter_edges_walk reread <adapters-file>  the same into adapters that are in use
 //        adapter_edges_walk stale <adapters-file>   a good file into adapters that hold a forward pass and gradients
 //        adapter_edges_walk empty                   a bunch without rows
+//        adapter_edges_walk inplace                 outputs that are inputs, of the adapters, RowTop and Distill
 #include <cstdio>
 #include <fstream>
 #include <iostream>
@@ -15,6 +16,7 @@
 #include "cudamatrix/cu-math.h"
 #include "nnet/nnet-adapters.h"
 #include "nnet/nnet-biasedlinearity.h"
+#include "nnet/nnet-loss.h"
 
 using namespace kaldi;
 
@@ -164,6 +166,28 @@ int Empty() {
   return 0;
 }
 
+int InPlace() {
+  Bench s;
+  CuMatrix<BaseFloat> out, y, val;
+  s.adapters.Propagate(&s.layer, s.x, s.who, KH_ACT_SIGMOID, &out);
+  const std::vector<float> x = Values(s.x), err = Values(s.err), o = Values(out);
+  y.CopyFromMat(s.x);
+  printf("propagate refused %d\n", Throws([&] { s.adapters.Propagate(&s.layer, s.x, s.who, KH_ACT_SIGMOID, &s.x); }));
+  printf("backpropagate refused %d %d %d\n", Throws([&] { s.adapters.Backpropagate(&s.layer, s.x, s.err, s.who, &y, &s.x); }),
+         Throws([&] { s.adapters.Backpropagate(&s.layer, s.x, s.err, s.who, &y, &s.err); }),
+         Throws([&] { s.adapters.Backpropagate(&s.layer, s.x, s.err, s.who, &y, &y); }));
+  CuStlVector<int32> id;
+  printf("row top refused %d\n", Throws([&] { cu::RowTop(out, 4, &id, &out, static_cast<CuVector<BaseFloat> *>(NULL)); }));
+  cu::RowTop(out, 4, &id, &val, static_cast<CuVector<BaseFloat> *>(NULL));
+  const std::vector<float> v = Values(val);
+  Distill loss(2.0, 0.0);
+  printf("distill refused %d\n", Throws([&] { loss.Eval(out, id, val, NULL, NULL, &val); }));
+  printf("inputs same %d\n", Values(s.x) == x && Values(s.err) == err && Values(out) == o && Values(y) == x && Values(val) == v);
+  loss.Eval(out, id, val, NULL, NULL, &out);  // (the gradient may take the logits' place)
+  printf("in place %d\n", Values(out) != o && out.NumRows() == s.kRows);
+  return 0;
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -172,9 +196,10 @@ int main(int argc, char **argv) {
     if (what == "read" && argc == 3) return Read(argv[2]);
     CuDevice::Instantiate().SelectGpuId(-1);
     if (what == "reread" && argc == 3) return Reread(argv[2]);
+    if (what == "inplace" && argc == 2) return InPlace();
     if (what == "empty" && argc == 2) return Empty();
     if (what == "stale" && argc == 3) return Stale(argv[2]);
-    fprintf(stderr, "usage: adapter_edges_walk read|reread|stale <adapters-file> | empty\n");
+    fprintf(stderr, "usage: adapter_edges_walk read|reread|stale <adapters-file> | empty | inplace\n");
     return 1;
   } catch (const std::exception &e) {
     std::cerr << e.what();

@@ -29,3 +29,11 @@ def test_a_bunch_without_rows(tmp_path):
     r = subprocess.run([WALK, "empty"], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stderr
     assert r.stdout.split("\n")[:4] == ["out 0 below 0 gradients zero 1", "out 37 below 37 gradients zero 0"] * 2
+
+
+def test_outputs_that_are_inputs(tmp_path):
+    """... are refused before they are resized: the inputs are still there."""
+    r = subprocess.run([WALK, "inplace"], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
+    assert r.stdout.split("\n")[:6] == ["propagate refused 1", "backpropagate refused 1 1 1", "row top refused 1", "distill refused 1",
+                                        "inputs same 1", "in place 1"]
