@@ -553,7 +553,7 @@ int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t K, int32_t
  * [0, cols) is none, its part of the row is zero.  w = weight[r] (NULL = 1); a row of weight 0, and a row whose x are
  * all -inf, get loss 0 and a gradient of zeros whatever the row holds.  row_loss (rows floats) may be NULL if loss is;
  * loss[0] += sum of row_loss (double on the device, summed in a fixed order: the same call gives the
- * same bits; may be NULL).  T > 0, 0 <= h <= 1.
+ * same bits; may be NULL).  2^-126 <= T (no subnormal float), 0 <= h <= 1.
  * Sums in float over at most 1024 partial sums per row, the logarithms in double.  At most 2^30 columns.  Uses no library
  * workspace. */
 int hipF_distill_eval(khStream_t s, const float *x, MatrixDim d, const int32_t *idx, int32_t ldidx, const float *val,

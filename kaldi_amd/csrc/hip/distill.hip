@@ -651,7 +651,8 @@ KH_EXPORT int hipF_distill_eval(khStream_t s, const float *x, MatrixDim d, const
   KH_REQUIRE(kh::dim_ok(d) && K >= 1 && ldidx >= K && ldval >= K);
   if (K > KH_MAX_TOP) return too_large(__func__, K);
   if (d.cols > kMaxCols) return too_wide(d.cols);
-  KH_REQUIRE(temperature > 0.f && temperature <= 3.402823466e38f);
+  // (the smallest normal float: log2(e) / T is a float then, and 0 / T a number)
+  KH_REQUIRE(temperature >= 1.17549435e-38f && temperature <= 3.402823466e38f);
   KH_REQUIRE(hard_weight >= 0.f && hard_weight <= 1.f);
   KH_REQUIRE(d.rows == 0 || (idx != nullptr && val != nullptr && (d.cols == 0 || x != nullptr)));
   KH_REQUIRE(d.rows == 0 || hard_weight == 0.f || label != nullptr);

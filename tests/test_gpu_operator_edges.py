@@ -111,3 +111,35 @@ def test_outputs_side_by_side_in_one_matrix(hip, N):
                  (gg[:, sgu], grads[3])):
         assert np.array_equal(a, b, equal_nan=True)
     assert np.isnan(got[:, [0, -2, -1]]).all() and np.isnan(gg[:, [0, -2, -1]]).all()
+
+
+@pytest.mark.parametrize("T", [2.0 ** -126, 1e-30, 1e30, 3.4e38])
+@pytest.mark.parametrize("C", [37, 1483, 30000])
+def test_distill_ends_of_the_temperature(hip, C, T):
+    """The softmax at the smallest temperature names the largest logit, at the largest all columns alike; nothing in between is
+    not a number.  Logits of -1, 0 and a single 1, weights that bring T (p - q) back to about 1."""
+    rs = np.random.RandomState(C)
+    R, K = 4, 3
+    x = -rs.randint(0, 2, (R, C)).astype(f32)
+    idx = np.stack([rs.permutation(C)[:K] for _ in range(R)])
+    val = np.tile(np.array([2, 1, 0], f32), (R, 1))
+    best = np.array([rs.randint(C) for _ in range(R)])
+    best[0], best[1] = idx[0, 0], idx[1, 2]
+    x[np.arange(R), best] = 1
+    weight = np.full(R, f32(2.0 ** -63) if T > 1 else f32(2.0 ** 63), f32)
+    m, di, dv = hip.DevMatrix.from_numpy(x), hip.DevMatrix.from_numpy(idx.astype(np.int32)), hip.DevMatrix.from_numpy(val)
+    dw = hip.DevMatrix.from_numpy(weight, False)
+    diff = hip.DevMatrix(R, C)
+    hip.call("hipF_distill_eval", None, m.ptr, m.dim, di.ptr, di.stride, dv.ptr, dv.stride, K, None, dw.ptr, T, 0.0, diff.ptr, diff.stride,
+             None, None)
+    p, q = np.zeros((R, C)), np.zeros((R, C))
+    if T < 1:
+        p[np.arange(R), best] = 1
+        q[np.arange(R), idx[:, 0]] = 1
+    else:
+        p[:] = 1.0 / C
+        np.put_along_axis(q, idx, 1.0 / K, 1)
+    ws = f64(weight[:, None]) * float(f32(T))
+    # p and q to 2^-17 of themselves (see test_gpu_distill.py), their product with w T and the difference to three roundings
+    tol = ws * (2.0 ** -17 + 3 * 2.0 ** -24) * (p + q) + 2.0 ** -126
+    assert (np.abs(diff.numpy() - ws * (p - q)) <= tol).all()

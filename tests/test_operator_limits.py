@@ -72,3 +72,9 @@ def test_distill_in_place_but_not_quite():
     # with the gradient in the logits' place, what lies over them lies over it
     assert status("hipF_distill_eval", a, diff=a["x"], row_loss=a["x"] + 4) == INVALID
     assert status("hipF_distill_eval", a, diff=a["x"], weight=a["x"] + 128 * 4 * 2) == INVALID
+
+
+@pytest.mark.parametrize("T", [2.0 ** -149, 1e-40, 2.0 ** -127])
+def test_distill_temperatures_whose_inverse_is_no_float(T):
+    assert status("hipF_distill_eval", APART["hipF_distill_eval"], temperature=T) == INVALID
+    assert b"temperature" in h.lib.hipK_error_string(INVALID)
