@@ -1100,7 +1100,15 @@ KH_EXPORT int hipF_softmax(khStream_t s, float *y, const float *x, MatrixDim d) 
   KH_REQUIRE(kh::dim_ok(d));
   if (d.rows == 0 || d.cols == 0) return KH_OK;
   KH_REQUIRE(y != nullptr && x != nullptr);
-  return kh::softmax_slabs_launch(kh::pick(s), y, d.stride, x, d.stride, 1, 0, nullptr, d.rows, d.cols, nullptr);
+  // a grid counts its threads in 32 bits (more are cut off without an error): up to 512 per row, so 2^21 rows at a time
+  constexpr int kRowsAtOnce = 1 << 21;
+  for (size_t r = 0; r < (size_t)d.rows; r += kRowsAtOnce) {
+    const int rows = d.rows - (int)r < kRowsAtOnce ? d.rows - (int)r : kRowsAtOnce;
+    const int rc = kh::softmax_slabs_launch(kh::pick(s), y + r * d.stride, d.stride, x + r * d.stride, d.stride, 1, 0, nullptr, rows,
+                                            d.cols, nullptr);
+    if (rc != KH_OK) return rc;
+  }
+  return KH_OK;
 }
 
 KH_EXPORT int hipF_softmax_part(khStream_t s, const float *X, const int32_t *vec_ids, float *Y, MatrixDim d) {

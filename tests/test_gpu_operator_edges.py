@@ -143,3 +143,20 @@ def test_distill_ends_of_the_temperature(hip, C, T):
     # p and q to 2^-17 of themselves (see test_gpu_distill.py), their product with w T and the difference to three roundings
     tol = ws * (2.0 ** -17 + 3 * 2.0 ** -24) * (p + q) + 2.0 ** -126
     assert (np.abs(diff.numpy() - ws * (p - q)) <= tol).all()
+
+
+@pytest.mark.parametrize("O", [2, 3])
+def test_softmax_layer_of_more_rows_than_one_launch_takes(hip, O):
+    """2^24 rows and more of a softmax output layer: rows of the softmax go in launches whose threads 32 bits count.  One input x
+    with weights 0, 1, ... and no bias: posteriors of exp(0), exp(x), ..., products of one and so exact up to the softmax (2^-20)."""
+    R = 2 ** 24 + 5
+    x = np.random.RandomState(O).randint(-64, 65, (R, 1)).astype(f32) / f32(32)
+    dx, dW = hip.DevMatrix.from_numpy(x, False), hip.DevMatrix.from_numpy(np.arange(O, dtype=f32)[:, None], False)
+    out = hip.DevMatrix(R, O, f32, False)
+    ad = hip.Adapters(0, 1, 0, None, None, None, 1, None, O)
+    hip.call("hipF_adapter_forward", None, hip.ACT_SOFTMAX, R, O, 1, dx.ptr, 1, dW.ptr, 1, None, ctypes.byref(ad), None, None, None, 0,
+             out.ptr, O)
+    z = x.astype(f64) * np.arange(O)
+    p = np.exp(z - z.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    assert (np.abs(out.numpy() - p) <= 2.0 ** -20 * p).all()
