@@ -497,7 +497,9 @@ int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int
  * together into tiles: give hipI32_adapter_plan's where neighbouring rows have different adapters, NULL where they lie
  * together already (utterances, single frames).  The result does not depend on it beyond rounding (a row that a broken
  * order does not list may stay unwritten).  `t` is what the backward pass needs; bias may be NULL.  out and t must
- * not overlap each other or an input (refused; matrices side by side in the rows of a larger one do not overlap).  Rows behind N and columns behind O (max_rank) are left as they are.  N <= 2^26; I, O <= 2^30.
+ * not overlap each other or an input (refused; matrices side by side in the rows of a larger one do not overlap).
+ * Rows behind N and columns behind O (max_rank) are left as they are; with O = 0 nothing is written.  N <= 2^26,
+ * I <= 2^30, O <= 2^29.
  * Uses no library workspace: may be captured into a graph.  A row of t has the same bits whoever shares its call, and
  * with hipK_gemm_row_invariant(1) so has a row of out.
  * Arithmetic: every float is taken as the sum of three bfloat16 numbers (24 bits of mantissa: exact) and a product
@@ -518,8 +520,8 @@ int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, int32_t I,
  * order / row_begin: hipI32_adapter_plan of the same rows; order must be a permutation of 0 .. N-1 for the
  * gradients to be whole (an entry outside is skipped).  An adapter without rows gets a gradient of zeros; rows of the
  * stacks outside every adapter are left as they are.  Sums are taken in a fixed order: the same call gives the same
- * bits.  Outputs must not overlap each other or an input that the call reads (refused).  N <= 2^26,
- * num * max(I, O) / 32 < 2^23 with gradients.  The shared W is not updated here (hipF_affine_update). */
+ * bits.  Outputs must not overlap each other or an input that the call reads (refused).  N <= 2^26, O <= 2^30,
+ * I <= 2^30 (2^29 with eout), num * max(I, O) / 32 < 2^23 with gradients.  The shared W is not updated here (hipF_affine_update). */
 int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t I, const float *e, int32_t lde, const float *in,
                           int32_t ldin, const float *W, int32_t ldw, const khAdapters *ad, const int32_t *row_adapter,
                           const int32_t *order, const int32_t *row_begin, const float *t, int32_t ldt, float *u,

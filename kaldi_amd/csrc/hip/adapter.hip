@@ -975,6 +975,13 @@ void launch_narrow(hipStream_t st, const NarrowArgs &p) {
   else narrow_kernel<2, VEC><<<grid, 64 * kNarrowWaves, 0, st>>>(p);
 }
 
+// The blocks of the narrow product in front of small tiles.  (a multiple of 8, so that the tiles still meet their dies; the blocks
+// too many are behind the last rank column)
+unsigned narrow_blocks_of(const WideArgs &p, const NarrowArgs &narrow) {
+  if (p.t == nullptr) return 0;
+  const int fn = p.st.max_rank <= 16 ? 1 : 2, windows = (p.N + narrow.window - 1) / narrow.window;
+  return (unsigned)(windows * ((p.st.max_rank + 16 * fn - 1) / (16 * fn)) + 7) / 8 * 8;
+}
 template <int MB, int NB, int NW, bool NN, bool VEC>
 void launch_wide_tile(hipStream_t st, WideArgs p, const NarrowArgs &narrow, FinishArgs *rest) {
   p.tiles_m = (p.N + 16 * MB - 1) / (16 * MB);
@@ -983,10 +990,8 @@ void launch_wide_tile(hipStream_t st, WideArgs p, const NarrowArgs &narrow, Fini
   if (p.t == nullptr) return wide_kernel<MB, NB, NW, NN, VEC, 0><<<blocks, 64 * NW, 0, st>>>(p, narrow, 0, 0);
   *rest = {p.N, p.C, p.t, p.ldt, p.side, p.ldside, p.st, p.row_adapter, p.y, p.ldy, p.act, p.out, p.ldout};
   p.y = nullptr, p.act = KH_ACT_NONE;
-  const int fn = p.st.max_rank <= 16 ? 1 : 2, windows = (p.N + narrow.window - 1) / narrow.window;
-  // (a multiple of 8, so that the tiles still meet their dies; the blocks too many are behind the last rank column)
-  const int narrow_blocks = (windows * ((p.st.max_rank + 16 * fn - 1) / (16 * fn)) + 7) / 8 * 8;
-  if (fn == 1) wide_kernel<MB, NB, NW, NN, VEC, 1><<<narrow_blocks + blocks, 64 * NW, 0, st>>>(p, narrow, windows, narrow_blocks);
+  const int windows = (p.N + narrow.window - 1) / narrow.window, narrow_blocks = (int)narrow_blocks_of(p, narrow);
+  if (p.st.max_rank <= 16) wide_kernel<MB, NB, NW, NN, VEC, 1><<<narrow_blocks + blocks, 64 * NW, 0, st>>>(p, narrow, windows, narrow_blocks);
   else wide_kernel<MB, NB, NW, NN, VEC, 2><<<narrow_blocks + blocks, 64 * NW, 0, st>>>(p, narrow, windows, narrow_blocks);
 }
 template <int WM, int WN, int MB, int NB, bool NN, bool VEC>
@@ -1003,27 +1008,36 @@ void launch_tiled(hipStream_t st, WideArgs p) {
 // 32x64 20); 256 rows 32x64 28 (16x32 38, 64x128 66); 1024 rows 64x128 73 (32x64 85, 128x128 101); 2048 rows 128x128 114 (64x128
 // 121, 256x128 167); 4096 rows 256x128 193 (128x128 220).
 template <bool NN, bool VEC>
-void launch_wide(hipStream_t st, const WideArgs &p, const NarrowArgs &narrow, FinishArgs *rest) {
-  static const struct { int rows, cols, round; } kTiles[] = {{16, 16, 7}, {16, 32, 11}, {32, 64, 21}, {64, 128, 62}, {128, 128, 95}, {256, 128, 170}};
+int launch_wide(hipStream_t st, const WideArgs &p, const NarrowArgs &narrow, FinishArgs *rest) {
+  static const struct { int rows, cols, round, threads; } kTiles[] = {{16, 16, 7, 512}, {16, 32, 11, 1024}, {32, 64, 21, 512},
+                                                                      {64, 128, 62, 512}, {128, 128, 95, 512}, {256, 128, 170, 512}};
   // (hipK_gemm_row_invariant: the tiled kernels only, which sum an element in the same order whatever their tile; so too where
-  // the small tiles' workgroups might be too many for a grid)
+  // the narrow product's workgroups might be too many in front of small tiles)
   const int first = kh::gemm_row_invariant() || p.N > (1 << 20) ? 3 : 0;
-  int best = first;
+  int best = -1;
   long long least = 0;
   for (int i = first; i < 6; ++i) {
-    const long long tiles = (long long)((p.N + kTiles[i].rows - 1) / kTiles[i].rows) * ((p.C + kTiles[i].cols - 1) / kTiles[i].cols);
-    const long long cost = (tiles + 255) / 256 * kTiles[i].round;
-    if (i == first || cost < least) best = i, least = cost;
+    const long long tiles_n = (p.C + kTiles[i].cols - 1) / kTiles[i].cols, tiles_m = (p.N + kTiles[i].rows - 1) / kTiles[i].rows;
+    const long long tiles = tiles_m * tiles_n, cost = (tiles + 255) / 256 * kTiles[i].round;
+    // a grid counts its threads in 32 bits (more are cut off without an error)
+    const long long blocks = i > 2 ? (tiles + 7) / 8 * 8 : (tiles_n + 7) / 8 * 8 * tiles_m + narrow_blocks_of(p, narrow);
+    if (blocks * kTiles[i].threads > 0xffffffffll) continue;
+    if (best < 0 || cost < least) best = i, least = cost;
+  }
+  if (best < 0) {
+    snprintf(kh::ctx().last_msg, sizeof(kh::ctx().last_msg), "%d rows of %d columns: too many tiles", p.N, p.C);
+    return KH_ERR_TOO_LARGE;
   }
   if (best > 2 && p.t) launch_narrow<VEC>(st, narrow);
   switch (best) {
-    case 0: return launch_wide_tile<1, 1, 8, NN, VEC>(st, p, narrow, rest);
-    case 1: return launch_wide_tile<1, 2, 16, NN, VEC>(st, p, narrow, rest);
-    case 2: return launch_wide_tile<2, 4, 8, NN, VEC>(st, p, narrow, rest);
-    case 3: return launch_tiled<2, 4, 1, 1, NN, VEC>(st, p);
-    case 4: return launch_tiled<4, 2, 1, 2, NN, VEC>(st, p);
-    default: return launch_tiled<4, 2, 2, 2, NN, VEC>(st, p);
+    case 0: launch_wide_tile<1, 1, 8, NN, VEC>(st, p, narrow, rest); break;
+    case 1: launch_wide_tile<1, 2, 16, NN, VEC>(st, p, narrow, rest); break;
+    case 2: launch_wide_tile<2, 4, 8, NN, VEC>(st, p, narrow, rest); break;
+    case 3: launch_tiled<2, 4, 1, 1, NN, VEC>(st, p); break;
+    case 4: launch_tiled<4, 2, 1, 2, NN, VEC>(st, p); break;
+    default: launch_tiled<4, 2, 2, 2, NN, VEC>(st, p);
   }
+  return kh::launch_status();
 }
 
 // A grid counts its threads in 32 bits: 2^26 rows in windows of 16 rows and 512 threads fill half of that.
@@ -1112,13 +1126,9 @@ KH_EXPORT int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, 
   WideArgs p = {in, ldin, W, ldw, N, I, O, bias, ad->num > 0 ? t : nullptr, ldt, ad->up, ad->ldup, stack, row_adapter, order,
                 nullptr, 0, act, out, ldout, 0, 0};
   FinishArgs rest = {};
-  if (vec) launch_wide<false, true>(st, p, na, &rest);
-  else launch_wide<false, false>(st, p, na, &rest);
-  if (rest.N > 0) {
-    rc = kh::launch_status();
-    if (rc != KH_OK) return rc;
-    launch_finish(st, rest);
-  }
+  rc = vec ? launch_wide<false, true>(st, p, na, &rest) : launch_wide<false, false>(st, p, na, &rest);
+  if (rc != KH_OK) return rc;
+  if (rest.N > 0) launch_finish(st, rest);
   rc = kh::launch_status();
   if (rc != KH_OK || act != KH_ACT_SOFTMAX) return rc;
   const MatrixDim d = {N, O, ldout};
@@ -1177,9 +1187,7 @@ KH_EXPORT int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t 
                   order, y, ldy, KH_ACT_NONE, eout, ldeout, 0, 0};
     const bool vec = vec_ok(e, lde) && vec_ok(W, ldw) && (ad->num == 0 || (vec_ok(ad->down, ad->lddown) &&
                      vec_ok(ad->up, ad->ldup) && vec_ok(u, ldu)));
-    if (vec) launch_wide<true, true>(st, p, na, &rest);
-    else launch_wide<true, false>(st, p, na, &rest);
-    rc = kh::launch_status();
+    rc = vec ? launch_wide<true, true>(st, p, na, &rest) : launch_wide<true, false>(st, p, na, &rest);
     if (rc != KH_OK) return rc;
   }
   if (cols == 0) {

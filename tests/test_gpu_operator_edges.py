@@ -160,3 +160,20 @@ def test_softmax_layer_of_more_rows_than_one_launch_takes(hip, O):
     p = np.exp(z - z.max(1, keepdims=True))
     p /= p.sum(1, keepdims=True)
     assert (np.abs(out.numpy() - p) <= 2.0 ** -20 * p).all()
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_a_row_of_almost_a_thousand_million_columns(hip, backward):
+    """Tiles by the million: as many threads as a grid counts.  One row of one input 1: out is the weights' column, bit by bit."""
+    h, C = hip, 2 ** 29
+    w = np.arange(C, dtype=np.int32).astype(f32)
+    dw, out, one = h.DevMatrix.from_numpy(w, False), h.DevMatrix(1, C, f32, False), h.DevMatrix.from_numpy(np.ones(1, f32), False)
+    ad = h.Adapters(0, 1, 0, None, None, None, 1, None, 1)
+    if backward:  # W is 1 x C: eout = e * W
+        h.call("hipF_adapter_backward", None, 1, 1, C, one.ptr, 1, None, 0, dw.ptr, C, ctypes.byref(ad), None, None, None, None, 0, None,
+               0, None, 0, out.ptr, C, None, 0, None, 0)
+    else:  # W is C x 1
+        h.call("hipF_adapter_forward", None, 0, 1, C, 1, one.ptr, 1, dw.ptr, 1, None, ctypes.byref(ad), None, None, None, 0, out.ptr, C)
+    assert np.array_equal(out.numpy()[0], w)
+    for m in (dw, out):
+        m.free()
