@@ -502,10 +502,12 @@ int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int
  * I <= 2^30, O <= 2^29.
  * Uses no library workspace: may be captured into a graph.  A row of t has the same bits whoever shares its call, and
  * with hipK_gemm_row_invariant(1) so has a row of out.
- * Arithmetic: every float is taken as the sum of three bfloat16 numbers (24 bits of mantissa: exact) and a product
- * of two floats as the six largest of the nine part products, on the matrix cores with float sums; what is left out
- * is below 2^-26 of the product, less than one rounding of a float product.  An infinity or NaN in a row of `in`
- * makes that row of t and out NaN (of `act` NaN); it does not reach other rows. */
+ * Arithmetic: every float is taken as the sum of three bfloat16 numbers (24 bits of mantissa: exact, the largest float
+ * included; below 2^-110 to 2^-134) and a product of two floats as the six largest of the nine part products, on the
+ * matrix cores with float sums; what is left out is below 2^-26 of the product (2^-25 beyond 0x1.fep127), less than one
+ * rounding of a float product.  A sum within 2^-7 of the largest float may come out infinite.  An infinity or NaN in a
+ * row of `in` makes that row of t and out NaN (of `act` NaN); it does not reach other rows.  A call takes up to twice
+ * as long where floats from 0x1.ffp127 on, infinities or NaN are among its operands. */
 int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, int32_t I, const float *in, int32_t ldin,
                          const float *W, int32_t ldw, const float *bias, const khAdapters *ad,
                          const int32_t *row_adapter, const int32_t *order, float *t, int32_t ldt, float *out,

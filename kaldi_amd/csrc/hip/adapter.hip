@@ -6,8 +6,10 @@
 // mantissa each, rounded to nearest: |x - hi| <= 2^-9 |x|, |x - hi - mid| <= 2^-18 |x|, the rest fits lo), and a product
 // is the sum of the six part products down to 2^-18 of it, accumulated in float by the matrix instruction: the bfloat16x3
 // decomposition published by Henry, Tang and Heinecke (2019).  The three products left out are at most
-// 2 * 2^-27 + 2^-36 of the product, an eighth of a float's rounding.  An infinity splits into inf + NaN.
+// 2 * 2^-27 + 2^-36 of the product, an eighth of a float's rounding.  An infinity splits into
+// inf + NaN; so does, at first, a finite float that rounds to infinity (first_part has what is done about it).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -33,9 +35,20 @@ __device__ __forceinline__ Minus minus_ones() {
   asm("" : "+s"(f), "+s"(s));
   return {__builtin_bit_cast(v2b, f), __builtin_bit_cast(v2b, s)};
 }
+// The first part.  What rounds to infinity, a finite float beyond the largest finite bfloat16, has a rest of minus infinity and
+// one of NaN: every sum that it is in is NaN.  CLAMP takes the largest finite bfloat16 instead, so that the rest is finite (that of
+// infinity is infinity, and the rest of that NaN).  It would be one instruction in seven more, 1 to 4 % of every call; so a
+// kernel goes over its operands without, and where a sum has come out as NaN, once more with it.
+template <bool CLAMP>
+__device__ __forceinline__ v2b first_part(float x, float y) {
+  constexpr float most = 0x1.fep+127f;
+  if (CLAMP) x = __builtin_amdgcn_fmed3f(x, -most, most), y = __builtin_amdgcn_fmed3f(y, -most, most);
+  return __builtin_convertvector((v2f){x, y}, v2b);
+}
+template <bool CLAMP>
 __device__ __forceinline__ void split2(float x, float y, v2b &hi, v2b &mid, v2b &lo) {
   const Minus one = minus_ones();
-  hi = __builtin_convertvector((v2f){x, y}, v2b);
+  hi = first_part<CLAMP>(x, y);
   x = __builtin_amdgcn_fdot2_f32_bf16(hi, one.first, x, false);
   y = __builtin_amdgcn_fdot2_f32_bf16(hi, one.second, y, false);
   mid = __builtin_convertvector((v2f){x, y}, v2b);
@@ -45,26 +58,36 @@ __device__ __forceinline__ void split2(float x, float y, v2b &hi, v2b &mid, v2b 
 }
 // the same with the parts unpacked and subtracted: where the matrix instructions keep the vector unit waiting anyway (the
 // tiled kernel), this measures 3 % faster than the above, in the kernels that split more than they multiply 6 % slower
+template <bool CLAMP>
 __device__ __forceinline__ void split2_apart(float x, float y, v2b &hi, v2b &mid, v2b &lo) {
-  hi = __builtin_convertvector((v2f){x, y}, v2b);
+  hi = first_part<CLAMP>(x, y);
   x -= (float)hi.x, y -= (float)hi.y;
   mid = __builtin_convertvector((v2f){x, y}, v2b);
   x -= (float)mid.x, y -= (float)mid.y;
   lo = __builtin_convertvector((v2f){x, y}, v2b);
 }
-template <bool APART = false>
+template <bool CLAMP = true, bool APART = false>
 __device__ __forceinline__ Frag split8(const float (&x)[8]) {
   Frag f;
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     v2b h, m, l;
-    if (APART) split2_apart(x[i], x[i + 1], h, m, l);
-    else split2(x[i], x[i + 1], h, m, l);
+    if (APART) split2_apart<CLAMP>(x[i], x[i + 1], h, m, l);
+    else split2<CLAMP>(x[i], x[i + 1], h, m, l);
     f.hi[i] = h.x, f.hi[i + 1] = h.y;
     f.mid[i] = m.x, f.mid[i + 1] = m.y;
     f.lo[i] = l.x, f.lo[i + 1] = l.y;
   }
   return f;
+}
+template <int N>
+__device__ __forceinline__ bool any_nan(const v4f (&v)[N]) {
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) nan |= v[j][i] != v[j][i];
+  return nan;
 }
 // c + small += a * b.  hi * hi has a sum of its own, which is then rounded once per step and not six times: what the matrix
 // instruction drops of a sum has a sign more often than not, and a gradient over many rows adds such errors up (8192 rows of
@@ -270,48 +293,52 @@ __device__ __forceinline__ void narrow_block(const NarrowArgs &p, int block_x, i
 #pragma unroll
     for (int j = 0; j < NB; ++j) br[j] = side + (size_t)(lo + min(col0 + NB * l15 + j, rank - 1)) * lds;
     v4f acc[NB], small[NB];
+    auto sweep = [&](auto clamp) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[j] = small[j] = (v4f){0.f, 0.f, 0.f, 0.f};
-    int k0 = 32 * wave;
-    if (VEC && k0 + 32 <= K) {
-      float *piece = sh.stage + wave * (16 + 16 * NB) * 32;
-      const float *sx[2], *sb[2 * NB];
+      for (int j = 0; j < NB; ++j) acc[j] = small[j] = (v4f){0.f, 0.f, 0.f, 0.f};
+      int k0 = 32 * wave;
+      if (VEC && k0 + 32 <= K) {
+        float *piece = sh.stage + wave * (16 + 16 * NB) * 32;
+        const float *sx[2], *sb[2 * NB];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sx[i] = x + (size_t)max(__shfl(row, 8 * i + (lane >> 3), 64), 0) * ldx;
+        for (int i = 0; i < 2; ++i) sx[i] = x + (size_t)max(__shfl(row, 8 * i + (lane >> 3), 64), 0) * ldx;
 #pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) {
-        const int r = 8 * i + (lane >> 3);  // piece row 16 j + l: the stack's row NB l + j
-        sb[i] = side + (size_t)(lo + min(col0 + NB * (r & 15) + (r >> 4), rank - 1)) * lds;
+        for (int i = 0; i < 2 * NB; ++i) {
+          const int r = 8 * i + (lane >> 3);  // piece row 16 j + l: the stack's row NB l + j
+          sb[i] = side + (size_t)(lo + min(col0 + NB * (r & 15) + (r >> 4), rank - 1)) * lds;
+        }
+        auto ask = [&](int k) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) stage_rows(sx[i] + k, lane, piece + 256 * i);
+#pragma unroll
+          for (int i = 0; i < 2 * NB; ++i) stage_rows(sb[i] + k, lane, piece + 512 + 256 * i);
+        };
+        ask(k0);
+        for (; k0 + 32 <= K; k0 += 32 * NW) {
+          float a[8], b[NB][8];
+          staged_arrived();
+          staged_row8(piece, l15, q, a);
+#pragma unroll
+          for (int j = 0; j < NB; ++j) staged_row8(piece + 512, 16 * j + l15, q, b[j]);
+          staged_taken();
+          if (k0 + 32 * NW + 32 <= K) ask(k0 + 32 * NW);
+          const Frag fa = split8<clamp.value>(a);
+#pragma unroll
+          for (int j = 0; j < NB; ++j) mfma6(fa, split8<clamp.value>(b[j]), acc[j], small[j]);
+        }
       }
-      auto ask = [&](int k) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) stage_rows(sx[i] + k, lane, piece + 256 * i);
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) stage_rows(sb[i] + k, lane, piece + 512 + 256 * i);
-      };
-      ask(k0);
-      for (; k0 + 32 <= K; k0 += 32 * NW) {
+      for (; k0 < K; k0 += 32 * NW) {
         float a[8], b[NB][8];
-        staged_arrived();
-        staged_row8(piece, l15, q, a);
+        load_row8<VEC>(xr + k0, q, K - k0, a);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) staged_row8(piece + 512, 16 * j + l15, q, b[j]);
-        staged_taken();
-        if (k0 + 32 * NW + 32 <= K) ask(k0 + 32 * NW);
-        const Frag fa = split8(a);
+        for (int j = 0; j < NB; ++j) load_row8<VEC>(br[j] + k0, q, K - k0, b[j]);
+        const Frag fa = split8<clamp.value>(a);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) mfma6(fa, split8(b[j]), acc[j], small[j]);
+        for (int j = 0; j < NB; ++j) mfma6(fa, split8<clamp.value>(b[j]), acc[j], small[j]);
       }
-    }
-    for (; k0 < K; k0 += 32 * NW) {
-      float a[8], b[NB][8];
-      load_row8<VEC>(xr + k0, q, K - k0, a);
-#pragma unroll
-      for (int j = 0; j < NB; ++j) load_row8<VEC>(br[j] + k0, q, K - k0, b[j]);
-      const Frag fa = split8(a);
-#pragma unroll
-      for (int j = 0; j < NB; ++j) mfma6(fa, split8(b[j]), acc[j], small[j]);
-    }
+    };
+    sweep(std::false_type());
+    if (__ballot(any_nan(small))) sweep(std::true_type());
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -393,10 +420,6 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p, NarrowArgs na
 #pragma unroll
   for (int b = 0; b < MB; ++b) xr[b] = p.x + (size_t)min(m0 + 16 * b + l15, p.N - 1) * p.ldx;
   v4f acc[MB][NB], small[MB][NB];
-#pragma unroll
-  for (int b = 0; b < MB; ++b)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) acc[b][j] = small[b][j] = (v4f){0.f, 0.f, 0.f, 0.f};
 
   const float *wr[NB];
 #pragma unroll
@@ -421,13 +444,13 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p, NarrowArgs na
       for (int j = 0; j < NB; ++j) load_row8<VEC>(wr[j] + k0, q, left, s.b[j]);
     }
   };
-  auto multiply = [&](const Step &s) {
+  auto multiply = [&](const Step &s, auto clamp) {
     Frag fa[MB];
 #pragma unroll
-    for (int m = 0; m < MB; ++m) fa[m] = split8(s.a[m]);
+    for (int m = 0; m < MB; ++m) fa[m] = split8<clamp.value>(s.a[m]);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const Frag fb = split8(s.b[j]);
+      const Frag fb = split8<clamp.value>(s.b[j]);
 #pragma unroll
       for (int m = 0; m < MB; ++m) mfma6(fa[m], fb, acc[m][j], small[m][j]);
     }
@@ -435,55 +458,66 @@ __global__ __launch_bounds__(64 * NW) void wide_kernel(WideArgs p, NarrowArgs na
   const int my_c = n0 + threadIdx.x % BN;
   const float my_bias = p.bias && my_c < p.C ? p.bias[my_c] : 0.f;  // for the end; asked for now
   constexpr int D = 32 * NW;
-  int k0 = 32 * wave;
-  if (VEC && k0 + 32 <= p.K) {
-    float *piece = stage_s + wave * STAGED * 32;
-    const float *sx[2 * MB], *sw[2 * NB];
+  auto sweep = [&](auto clamp) {
 #pragma unroll
-    for (int i = 0; i < 2 * MB; ++i) sx[i] = p.x + (size_t)min(m0 + 8 * i + (lane >> 3), p.N - 1) * p.ldx;
+    for (int m = 0; m < MB; ++m)
 #pragma unroll
-    for (int i = 0; i < 2 * NB; ++i) {
-      const int r = 8 * i + (lane >> 3);  // piece row 16 j + l: row NB l + j of the tile's part of W
-      sw[i] = p.w + (size_t)min(n0 + NB * (r & 15) + (r >> 4), p.C - 1) * p.ldw;
-    }
-    float raw[8][NB];  // (NN: rows of W along the tile's columns, straight into registers)
-    auto ask = [&](int k) {
+      for (int j = 0; j < NB; ++j) acc[m][j] = small[m][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    int k0 = 32 * wave;
+    if (VEC && k0 + 32 <= p.K) {
+      float *piece = stage_s + wave * STAGED * 32;
+      const float *sx[2 * MB], *sw[2 * NB];
 #pragma unroll
-      for (int i = 0; i < 2 * MB; ++i) stage_rows(sx[i] + k, lane, piece + 256 * i);
-      if (NN) {
-        const float *w = p.w + (size_t)k * p.ldw;
+      for (int i = 0; i < 2 * MB; ++i) sx[i] = p.x + (size_t)min(m0 + 8 * i + (lane >> 3), p.N - 1) * p.ldx;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) load_cols<NB, VEC>(w + (size_t)inner(q, e) * p.ldw, c0, p.C, raw[e]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) stage_rows(sw[i] + k, lane, piece + 512 * MB + 256 * i);
+      for (int i = 0; i < 2 * NB; ++i) {
+        const int r = 8 * i + (lane >> 3);  // piece row 16 j + l: row NB l + j of the tile's part of W
+        sw[i] = p.w + (size_t)min(n0 + NB * (r & 15) + (r >> 4), p.C - 1) * p.ldw;
       }
-    };
-    ask(k0);
-    for (; k0 + 32 <= p.K; k0 += D) {
-      Step s;
-      staged_arrived();
+      float raw[8][NB];  // (NN: rows of W along the tile's columns, straight into registers)
+      auto ask = [&](int k) {
 #pragma unroll
-      for (int m = 0; m < MB; ++m) staged_row8(piece, 16 * m + l15, q, s.a[m]);
-      if (NN) {
+        for (int i = 0; i < 2 * MB; ++i) stage_rows(sx[i] + k, lane, piece + 256 * i);
+        if (NN) {
+          const float *w = p.w + (size_t)k * p.ldw;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+          for (int e = 0; e < 8; ++e) load_cols<NB, VEC>(w + (size_t)inner(q, e) * p.ldw, c0, p.C, raw[e]);
+        } else {
 #pragma unroll
-          for (int j = 0; j < NB; ++j) s.b[j][e] = raw[e][j];
-      } else {
+          for (int i = 0; i < 2 * NB; ++i) stage_rows(sw[i] + k, lane, piece + 512 * MB + 256 * i);
+        }
+      };
+      ask(k0);
+      for (; k0 + 32 <= p.K; k0 += D) {
+        Step s;
+        staged_arrived();
 #pragma unroll
-        for (int j = 0; j < NB; ++j) staged_row8(piece + 512 * MB, 16 * j + l15, q, s.b[j]);
+        for (int m = 0; m < MB; ++m) staged_row8(piece, 16 * m + l15, q, s.a[m]);
+        if (NN) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) s.b[j][e] = raw[e][j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < NB; ++j) staged_row8(piece + 512 * MB, 16 * j + l15, q, s.b[j]);
+        }
+        staged_taken();
+        if (k0 + D + 32 <= p.K) ask(k0 + D);
+        multiply(s, clamp);
       }
-      staged_taken();
-      if (k0 + D + 32 <= p.K) ask(k0 + D);
-      multiply(s);
     }
-  }
-  for (; k0 < p.K; k0 += D) {
-    Step rest;
-    load(k0, p.K - k0, rest);
-    multiply(rest);
-  }
+    for (; k0 < p.K; k0 += D) {
+      Step rest;
+      load(k0, p.K - k0, rest);
+      multiply(rest, clamp);
+    }
+  };
+  sweep(std::false_type());
+  bool nan = false;
+#pragma unroll
+  for (int m = 0; m < MB; ++m) nan |= any_nan(small[m]);
+  if (__ballot(nan)) sweep(std::true_type());
 
   __syncthreads();  // (the pieces of LDS have been read: now they take the sums)
   constexpr int EACH = BM * BN / (64 * NW) > 0 ? BM * BN / (64 * NW) : 1;
@@ -586,11 +620,12 @@ __device__ __forceinline__ v16f mfma6_32(const Frag &a, const Frag &b, v16f c) {
 }
 
 // four floats as three times four bfloat16
+template <bool CLAMP>
 __device__ __forceinline__ void split4(v4f x, v4b &hi, v4b &mid, v4b &lo) {
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
     v2b h, m, l;
-    split2_apart(x[i], x[i + 1], h, m, l);
+    split2_apart<CLAMP>(x[i], x[i + 1], h, m, l);
     hi[i] = h.x, hi[i + 1] = h.y;
     mid[i] = m.x, mid[i + 1] = m.y;
     lo[i] = l.x, lo[i + 1] = l.y;
@@ -675,12 +710,12 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
       for (int e = 0; e < 8; ++e) rc[u][e] = k0 + 8 * kc + e < p.K ? bc[u][(size_t)(k0 + e) * p.ldw] : 0.f;
     }
   };
-  auto put = [&](int buf) {
+  auto put = [&](int buf, auto clamp) {
     const int kc = ka >> 3, sub = ka & 4;
 #pragma unroll
     for (int u = 0; u < AU; ++u) {
       v4b h, m, l;
-      split4(ra[u], h, m, l);
+      split4<clamp.value>(ra[u], h, m, l);
       const int s = slot_of((tid >> 3) + 64 * u, kc);
       *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][0][s]) + sub) = h;
       *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][1][s]) + sub) = m;
@@ -689,7 +724,7 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
 #pragma unroll
     for (int u = 0; u < BU; ++u) {
       v4b h, m, l;
-      split4(rb[u], h, m, l);
+      split4<clamp.value>(rb[u], h, m, l);
       const int s = A_SLOTS + slot_of((tid >> 3) + 64 * u, kc);
       *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][0][s]) + sub) = h;
       *reinterpret_cast<v4b *>(reinterpret_cast<__bf16 *>(&lds[buf][1][s]) + sub) = m;
@@ -699,7 +734,7 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
     for (int u = 0; u < BC; ++u) {
       const int n = (tid + 512 * u) % BN, c = (tid + 512 * u) / BN;
       if (c < 4) {
-        const Frag f = split8<true>(rc[u]);
+        const Frag f = split8<clamp.value, true>(rc[u]);
         const int s = A_SLOTS + slot_of(n, c);
         lds[buf][0][s] = f.hi, lds[buf][1][s] = f.mid, lds[buf][2][s] = f.lo;
       }
@@ -709,13 +744,6 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
   // hi * hi is summed apart from the five small part products: the large sum is then rounded once per instruction of its
   // own, not six times (relative error over 2048 products 3e-7 instead of 9e-7)
   v16f acc[MB][NB], rest_of[MB][NB];
-#pragma unroll
-  for (int m = 0; m < MB; ++m)
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[m][n][i] = rest_of[m][n][i] = 0.f;
-
   const int steps = (p.K + 31) / 32;
   // the products of one half of a step: the six part products in turn, each over all blocks (a block's sum is then
   // not waited for)
@@ -740,30 +768,47 @@ __global__ __launch_bounds__(512) void tiled_kernel(WideArgs p) {
           sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[m][pa[q]], fb[n][pb[q]], sum, 0, 0, 0);
         }
   };
-  if (steps > 0) {
-    fetch(0);
-    put(0);
-    if (steps > 1) fetch(32);
-    __syncthreads();
-  }
-  int s = 0;
-  if (VEC)
-    for (; 32 * (s + 3) <= p.K; ++s) {
+  auto sweep = [&](auto clamp) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[m][n][i] = rest_of[m][n][i] = 0.f;
+    if (steps > 0) {
+      fetch(0);
+      put(0, clamp);
+      if (steps > 1) fetch(32);
+      __syncthreads();
+    }
+    int s = 0;
+    if (VEC)
+      for (; 32 * (s + 3) <= p.K; ++s) {
+        const int buf = s & 1;
+        multiply(buf, 0);
+        put(buf ^ 1, clamp);
+        fetch_whole(32 * (s + 2));
+        multiply(buf, 1);
+        __syncthreads();
+      }
+    for (; s < steps; ++s) {
       const int buf = s & 1;
       multiply(buf, 0);
-      put(buf ^ 1);
-      fetch_whole(32 * (s + 2));
+      if (s + 1 < steps) put(buf ^ 1, clamp);
+      if (s + 2 < steps) fetch(32 * (s + 2));
       multiply(buf, 1);
       __syncthreads();
     }
-  for (; s < steps; ++s) {
-    const int buf = s & 1;
-    multiply(buf, 0);
-    if (s + 1 < steps) put(buf ^ 1);
-    if (s + 2 < steps) fetch(32 * (s + 2));
-    multiply(buf, 1);
-    __syncthreads();
-  }
+  };
+  sweep(std::false_type());
+  bool nan = false;
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) nan |= rest_of[m][n][i] != rest_of[m][n][i];
+  if (__syncthreads_or(nan)) sweep(std::true_type());
 
 #pragma unroll
   for (int m = 0; m < MB; ++m)
@@ -869,36 +914,43 @@ __global__ __launch_bounds__(64 * NW) void grad_kernel(GradArgs down, GradArgs u
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, q = lane >> 4;
   const int begin = min(max(row_begin[g], 0), N), end = min(row_begin[g + 1], N), c0 = n0 + NB * l15;
   v4f acc[MB][NB], small[MB][NB];
+  auto sweep = [&](auto clamp) {
 #pragma unroll
-  for (int m = 0; m < MB; ++m)
+    for (int m = 0; m < MB; ++m)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[m][j] = small[m][j] = (v4f){0.f, 0.f, 0.f, 0.f};
-  int mine = begin + 32 * wave + lane < end && lane < 32 ? row_of(order, begin + 32 * wave + lane, N) : -1;
-  for (int r0 = begin + 32 * wave; r0 < end; r0 += 32 * NW) {
-    float a[MB][8], b[NB][8];
+      for (int j = 0; j < NB; ++j) acc[m][j] = small[m][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    int mine = begin + 32 * wave + lane < end && lane < 32 ? row_of(order, begin + 32 * wave + lane, N) : -1;
+    for (int r0 = begin + 32 * wave; r0 < end; r0 += 32 * NW) {
+      float a[MB][8], b[NB][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int r = __shfl(mine, inner(q, e), 64);
+      for (int e = 0; e < 8; ++e) {
+        const int r = __shfl(mine, inner(q, e), 64);
 #pragma unroll
-      for (int m = 0; m < MB; ++m)
-        a[m][e] = r >= 0 && k_base + 16 * m + l15 < rank ? p.narrow[(size_t)r * p.ldnarrow + k_base + 16 * m + l15] : 0.f;
-      float v[NB] = {};
-      if (r >= 0) load_cols<NB, VEC>(p.wide + (size_t)r * p.ldwide, c0, p.C, v);
+        for (int m = 0; m < MB; ++m)
+          a[m][e] = r >= 0 && k_base + 16 * m + l15 < rank ? p.narrow[(size_t)r * p.ldnarrow + k_base + 16 * m + l15] : 0.f;
+        float v[NB] = {};
+        if (r >= 0) load_cols<NB, VEC>(p.wide + (size_t)r * p.ldwide, c0, p.C, v);
 #pragma unroll
-      for (int j = 0; j < NB; ++j) b[j][e] = v[j];
+        for (int j = 0; j < NB; ++j) b[j][e] = v[j];
+      }
+      const int later = r0 + 32 * NW + lane;
+      mine = later < end && lane < 32 ? row_of(order, later, N) : -1;
+      Frag fa[MB];
+#pragma unroll
+      for (int m = 0; m < MB; ++m) fa[m] = split8<clamp.value>(a[m]);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const Frag fb = split8<clamp.value>(b[j]);
+#pragma unroll
+        for (int m = 0; m < MB; ++m) mfma6(fa[m], fb, acc[m][j], small[m][j]);
+      }
     }
-    const int later = r0 + 32 * NW + lane;
-    mine = later < end && lane < 32 ? row_of(order, later, N) : -1;
-    Frag fa[MB];
+  };
+  sweep(std::false_type());
+  bool nan = false;
 #pragma unroll
-    for (int m = 0; m < MB; ++m) fa[m] = split8(a[m]);
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const Frag fb = split8(b[j]);
-#pragma unroll
-      for (int m = 0; m < MB; ++m) mfma6(fa[m], fb, acc[m][j], small[m][j]);
-    }
-  }
+  for (int m = 0; m < MB; ++m) nan |= any_nan(small[m]);
+  if (__ballot(nan)) sweep(std::true_type());
 #pragma unroll
   for (int m = 0; m < MB; ++m)
 #pragma unroll

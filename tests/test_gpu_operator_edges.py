@@ -5,7 +5,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from test_gpu_adapters import Case, bound, within
+from test_gpu_adapters import Case, bound, check_backward, within
 from test_gpu_distill import check_distill
 
 pytestmark = pytest.mark.gpu
@@ -177,3 +177,53 @@ def test_a_row_of_almost_a_thousand_million_columns(hip, backward):
     assert np.array_equal(out.numpy()[0], w)
     for m in (dw, out):
         m.free()
+
+
+LARGEST = np.array([np.finfo(f32).max, np.finfo(f32).min, float.fromhex("0x1.ffp127"), float.fromhex("-0x1.ffp127"),
+                    float.fromhex("0x1.fefffep127"), float.fromhex("0x1.fep127")], f32)  # around where bfloat16 ends
+# which operand holds the largest floats, and what is scaled down so that the sums stay finite
+SCALED = {"x": "W down e", "W": "x e", "down": "x e", "up": "x e", "e": "W up x", "t": "x e"}
+
+
+@pytest.mark.parametrize("where", sorted(SCALED))
+@pytest.mark.parametrize("shape", [
+    (1, 33, 70, 2, 5, "each"), (17, 130, 100, 7, 33, "each"), (64, 259, 440, 80, 32, "each"), (300, 512, 511, 3, 128, "segments"),
+    (1000, 320, 256, 500, 7, "shuffled"), (2000, 2048, 40, 12, 33, "segments"), (2000, 40, 2048, 12, 33, "segments"),
+    (4000, 2048, 36, 12, 128, "shuffled"), (4000, 36, 2048, 12, 128, "shuffled")])
+def test_the_largest_floats(hip, shape, where):
+    """Finite floats that round to an infinite bfloat16 are floats like any other: the tolerances of test_gpu_adapters.py."""
+    c = Case(hip, *shape, seed=sum(shape[:5]), none=0.0)
+    rs = np.random.RandomState(sum(shape[:5]))
+    for name in SCALED[where].split():
+        getattr(c, name)[:] *= f32(2.0 ** -60)
+    t = c.forward(0)[1].astype(f32)
+    a = t if where == "t" else getattr(c, where)
+    hit = rs.rand(*a.shape) < 0.03
+    hit.flat[rs.randint(a.size)] = True
+    if where == "t":  # (what lies behind an adapter's rank is not read)
+        t *= f32(2.0 ** -60)
+    a[hit] = rs.choice(LARGEST, hit.sum())
+    if where != "t":
+        t = c.forward(0)[1].astype(f32)
+        out, got_t = c.run_forward(0, True)
+        want, t64, mag, tmag = c.forward(0)
+        within(got_t, t64, bound(c.I) * tmag + 1e-37)
+        within(out, want, (bound(c.I, c.rank) + bound(c.I)) * mag + 1e-37)
+    check_backward(c, t, with_y=False)
+
+
+def test_infinities_beside_the_largest_floats(hip):
+    """... stay what they were: NaN in their rows, the others as they are."""
+    for N, O, I in ((40, 70, 64), (300, 70, 64), (4000, 300, 64)):
+        c = Case(hip, N, O, I, 6, 8, "shuffled", seed=9, ragged=False, none=0.2)
+        c.W *= f32(2.0 ** -60)
+        c.down *= f32(2.0 ** -60)
+        c.x[::3, 5] = np.finfo(f32).max
+        good_out, good_t = c.run_forward(0, True)
+        assert np.isfinite(good_out).all() and np.isfinite(good_t).all()
+        c.x[17, 3] = np.inf
+        c.x[33, 3] = np.nan
+        out, t = c.run_forward(0, True)
+        rest = np.setdiff1d(np.arange(N), [17, 33])
+        assert np.array_equal(out[rest], good_out[rest]) and np.array_equal(t[rest], good_t[rest])
+        assert np.isnan(out[[17, 33]]).all()
