@@ -227,3 +227,76 @@ def test_infinities_beside_the_largest_floats(hip):
         rest = np.setdiff1d(np.arange(N), [17, 33])
         assert np.array_equal(out[rest], good_out[rest]) and np.array_equal(t[rest], good_t[rest])
         assert np.isnan(out[[17, 33]]).all()
+
+
+class Strided:
+    """A matrix whose rows are far apart; its last rows begin behind 2^31 elements."""
+
+    def __init__(self, h, a, stride):
+        self.h, self.shape, self.stride, self.dtype = h, a.shape, stride, a.dtype
+        self.m = h.DevMatrix((a.shape[0] - 1) * stride + a.shape[1], 1, a.dtype, False, False)
+        self.ptr = self.m.ptr
+        self.copy(np.ascontiguousarray(a), 0)
+
+    def copy(self, a, kind):
+        es = self.dtype.itemsize
+        host, dev = (a.ctypes.data_as(ctypes.c_void_p), a.shape[1] * es), (self.ptr, self.stride * es)
+        self.h.synchronize()
+        self.h.call("hipK_memcpy_2d", None, *(dev + host if kind == 0 else host + dev), a.shape[1] * es, a.shape[0], kind)
+        return a
+
+    def numpy(self):
+        return self.copy(np.empty(self.shape, self.dtype), 1)
+
+
+@pytest.mark.parametrize("invariant", [0, 1])
+@pytest.mark.parametrize("stride", [700000000, 700000001])
+def test_adapters_strides_that_pass_32_bits(hip, stride, invariant):
+    """Small tiles and (rows independent of the bunch) large ones, aligned rows and others, every matrix with rows 2.8 GB apart: the
+    same as with rows close together, to the tolerances of test_gpu_adapters.py."""
+    h = hip
+    c = Case(h, 5, 5, 5, 2, 3, "each", ragged=False, seed=8, none=0.0)
+    want_out, _, mag, _ = c.forward(0)
+    h.call("hipK_gemm_row_invariant", invariant)
+    try:
+        put = lambda a: Strided(h, a, stride)  # noqa: E731
+        x, W, e, down, up = put(c.x), put(c.W), put(c.e), put(c.down[:6]), put(c.up[:6])
+        blank = lambda r, n: put(np.full((r, n), np.nan, f32))  # noqa: E731
+        t, out, u, eout, gd, gu = blank(5, 3), blank(5, 5), blank(5, 3), blank(5, 5), blank(6, 5), blank(6, 5)
+        ad = h.Adapters(2, 3, 6, c.vec(c.begin).value, c.vec(c.scale).value, down.ptr.value, stride, up.ptr.value, stride)
+        ids, order, begin = c.vec(c.ids), c.vec(c.order), c.vec(c.row_begin)
+        h.call("hipF_adapter_forward", None, 0, 5, 5, 5, x.ptr, stride, W.ptr, stride, c.vec(c.bias), ctypes.byref(ad), ids, order, t.ptr,
+               stride, out.ptr, stride)
+        within(out.numpy(), want_out, (bound(5, 3) + bound(5)) * mag)
+        h.call("hipF_adapter_backward", None, 5, 5, 5, e.ptr, stride, x.ptr, stride, W.ptr, stride, ctypes.byref(ad), ids, order, begin,
+               t.ptr, stride, u.ptr, stride, None, 0, eout.ptr, stride, gd.ptr, stride, gu.ptr, stride)
+        got = [m.numpy() for m in (u, eout, gd, gu)]
+        c.run_backward = lambda *a: [got[0], got[1]] + [np.vstack([g, np.full((2, 5), np.nan, f32)]) for g in got[2:]]
+        check_backward(c, t.numpy(), with_y=False)
+    finally:
+        h.call("hipK_gemm_row_invariant", 0)
+
+
+@pytest.mark.parametrize("stride", [700000000, 700000001])
+@pytest.mark.parametrize("C", [50, 25000])
+def test_top_and_distill_strides_that_pass_32_bits(hip, stride, C):
+    h, rs = hip, np.random.RandomState(C)
+    R, K = 5, 4
+    x = rs.randn(R, C).astype(f32)
+    m = Strided(h, x, stride)
+    idx, val = Strided(h, np.zeros((R, K), np.int32), stride), Strided(h, np.zeros((R, K), f32), stride)
+    h.call("hipF_row_top", None, m.ptr, h.MatrixDim(R, C, stride), K, idx.ptr, stride, val.ptr, stride, None)
+    at = np.argsort(-x, 1, kind="stable")[:, :K]
+    assert np.array_equal(idx.numpy(), at) and np.array_equal(val.numpy(), np.take_along_axis(x, at, 1))
+    z = rs.randn(R, C).astype(f32)
+    near = h.DevMatrix.from_numpy(z), h.DevMatrix.from_numpy(at.astype(np.int32)), h.DevMatrix.from_numpy(val.numpy()), h.DevMatrix(R, C)
+    far = Strided(h, z, stride), idx, val, Strided(h, np.zeros((R, C), f32), stride)
+    loss = [h.DevMatrix(1, R, f32, False) for _ in range(2)]
+    for (a, i, v, d), r in zip((near, far), loss):
+        h.call("hipF_distill_eval", None, a.ptr, h.MatrixDim(R, C, a.stride), i.ptr, i.stride, v.ptr, v.stride, K, None, None, 2.0, 0.0, d.ptr,
+               d.stride, r.ptr, None)
+    if stride % 4 == 0:  # (other rows are summed in another order)
+        assert np.array_equal(near[3].numpy(), far[3].numpy()) and np.array_equal(loss[0].numpy(), loss[1].numpy())
+    else:  # two results, each good to 2^-17 + 2^-24 * 10 of the probabilities times T
+        assert np.abs(near[3].numpy() - far[3].numpy()).max() <= 2 * 2 * 2.0 ** -16
+        assert np.abs(loss[0].numpy() - loss[1].numpy()).max() <= 2 * 9 * 2.0 ** -18 + 2.0 ** -20
