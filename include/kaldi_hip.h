@@ -495,8 +495,8 @@ int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int
  *   out(N x O)       out[r,:] = act( bias + in[r,:] * W^T + t[r,:] * up_g )
  * with g = row_adapter[r].  `order` (may be NULL: the rows as they stand) is the sequence in which rows are put
  * together into tiles: give hipI32_adapter_plan's where neighbouring rows have different adapters, NULL where they lie
- * together already (utterances, single frames).  The result does not depend on it beyond rounding (a row that a broken
- * order does not list may stay unwritten).  `t` is what the backward pass needs; bias may be NULL.  out and t must
+ * together already (utterances, single frames).  The result does not depend on it beyond rounding (t and out of a row
+ * that a broken order does not list are undefined).  `t` is what the backward pass needs; bias may be NULL.  out and t must
  * not overlap each other or an input (refused; matrices side by side in the rows of a larger one do not overlap).
  * Rows behind N and columns behind O (max_rank) are left as they are; with O = 0 nothing is written.  N <= 2^26,
  * I <= 2^30, O <= 2^29.
@@ -553,7 +553,8 @@ int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t K, int32_t
  *   diff     = w * [ (1-h) * T * (p * (1 if there is an entry else 0) - q)  +  h * (p1 - onehot(label)) ]
  * diff is the derivative of row_loss with respect to x; it may be NULL (the loss alone) or be x
  * itself (same stride); else no output may overlap another or an input (refused).  A column named by two
- * entries gets both; an entry of -inf has q = 0 and 0 * log 0 = 0.  label (may be NULL when h is 0): a label outside
+ * entries gets both; an entry of -inf has q = 0 and 0 * log 0 = 0 (a row of nothing else has no
+ * entry).  label (may be NULL when h is 0): a label outside
  * [0, cols) is none, its part of the row is zero.  w = weight[r] (NULL = 1); a row of weight 0, and a row whose x are
  * all -inf, get loss 0 and a gradient of zeros whatever the row holds.  row_loss (rows floats) may be NULL if loss is;
  * loss[0] += sum of row_loss (double on the device, summed in a fixed order: the same call gives the

@@ -1,9 +1,13 @@
 // Learning from another network's outputs: hipF_row_top (a row's largest logits) and hipF_distill_eval (loss and gradient
 // towards them, mixed with hard labels); include/kaldi_hip.h has the formulas.
 //
-// Both are bound by reading (and writing) the logits once.  A row is one workgroup's, whose threads hold up to kHold floats
-// of it each: up to 1024 * kHold = 20480 columns stay in registers between the maximum, the sum and the output, and longer
-// rows are gone through in such chunks.
+// A row is one workgroup's, whose threads hold up to kHold floats of it each: up to 1024 * kHold = 20480 columns stay in
+// registers between the maximum, the sum and the output, so that the logits are read (and their gradient written) once.  Longer
+// rows are gone through in such chunks, by hipF_row_top once, by hipF_distill_eval with a gradient twice: the sums have to be
+// whole before the first column can be written.
+//
+// Memory rates that the figures below compare with (calls in a row, operands in turn that the last-level cache does not hold):
+// this library's column sums read 0.3 to 4 GB at 5.9 to 6.0 TB/s, its sigmoid copies 300 to 600 MB at 6.2 and 2 to 4 GB at 5.1.
 #include <algorithm>
 
 #include "common.h"
@@ -141,7 +145,8 @@ __device__ __forceinline__ key_t key_of(float x, int c) { return (key_t)ordered(
 constexpr int kCap = 1024;  // candidates of a chunk, next to the KH_MAX_TOP of the chunks before
 
 // AHEAD false: a workgroup has one row, of one chunk; 64 registers, so that eight waves share a SIMD and hide each other's
-// loads (4096 rows of 9000, K 32: 36.7 us, 4.0 TB/s, what a plain sum of as much memory reads at).  AHEAD: rows of several
+// loads (4096 rows of 9000, K 32: 36.7 us, 4.0 TB/s, two thirds of what column sums read at; the vector units are busy for 56 % of
+// that, and a workgroup asks for nothing more while it works on its row).  AHEAD: rows of several
 // chunks of equal length; a workgroup takes one row after another and has the next chunk loaded into LDS while it works on one
 // in registers, a wave waiting for its own part only (256 rows of 70001, K 64: 24.1 us, 25.0 with whole chunks and a rest;
 // short rows measure 44 us that way).
@@ -149,7 +154,10 @@ constexpr int kCap = 1024;  // candidates of a chunk, next to the KH_MAX_TOP of 
 // chunk's K-th largest, and where large values are spread over the row few more than K elements reach the best such value.
 // It is found by bisection to K .. 1.25 K groups, every wave for itself.  (Later chunks: the K-th largest so far.)  The
 // elements that reach the bound are collected in LDS and ranked by counting; the K largest are kept.  Where more than kCap reach the bound (large values crowded into few groups, many equal ones), and
-// where the chunk holds a NaN or +inf, a bound on the distinct keys is found by bisection over the chunk.
+// where the chunk holds a NaN or +inf, or fewer than K groups a number, a bound on the distinct keys is found by bisection over
+// the chunk, which is read again from the caches in every round.  That is slow: 4096 rows of 9000, K 32, of one value or nearly all
+// -inf 1.4 ms, of eight values 0.56 ms, with one NaN or +inf each 0.12 ms, in ascending order (no search) 66 us; 256 rows of 70001, K 64:
+// 0.77 to 0.80 ms, 0.73 ms, 47 us, 0.19 ms.
 template <int THREADS, bool VEC, bool AHEAD>
 __global__ __launch_bounds__(THREADS, AHEAD ? 4 : THREADS == 64 ? 3 : 8) void row_top_kernel(const float *mat, MatrixDim d, int K, int32_t *idx, int ldidx,
                                                           float *val, int ldval, float *lse) {
@@ -377,8 +385,9 @@ struct DistillArgs {
 // them; the gradient is written from the exponentials in registers, and after a second barrier the few columns that the
 // teacher or the label names are written once more with their targets taken off.  The first wave works out the teacher's
 // distribution, the last one those columns.  A row of several chunks is read twice.  BOTH: the sums at temperature T and
-// at 1 are needed.  4096 rows of 9000 with their gradient: 62.9 us, 4.7 TB/s, the rate of a large copy; the loss alone of
-// 1999 such rows: 18.4 us, 3.9 TB/s.  (Rows loaded ahead through LDS as above: 87 and 28 us, fewer waves at a time.)
+// at 1 are needed.  4096 rows of 9000 with their gradient: 62.8 us, 4.7 TB/s, three quarters of an
+// elementwise pass's rate; the loss alone of 1999 such rows: 18.2 us, 4.0 TB/s, two thirds of a sum's; 70001 columns, read twice by one
+// workgroup per row: 1 row 22 us, 64 rows 25, 256 rows 37.  (Rows loaded ahead through LDS as above: 87 and 28 us, fewer waves at a time.)
 template <int THREADS, bool VEC, bool BOTH>
 __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs p) {
   constexpr int waves = THREADS / 64, chunk = THREADS * kHold;
@@ -556,6 +565,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs p) {
   }
 }
 
+// One workgroup behind the rows' (256 rows 1.8 us, 4096 rows 3 to 4, 2^25 rows 47 ms).
 // loss[0] += the rows' losses, in a fixed order: thread t adds rows t, t + 256, ..., then the threads' sums in a tree
 __global__ __launch_bounds__(256) void sum_rows_kernel(const float *row_loss, int rows, double *loss) {
   __shared__ double sd[4];
