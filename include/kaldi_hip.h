@@ -482,10 +482,10 @@ typedef struct {
 
 /* Groups the N rows of a bunch by adapter: order[] lists the rows of adapter 0, then of adapter 1, ..., each in
  * ascending order, then the rows without one (row_adapter[r] outside [0, num)); adapter g's are
- * order[row_begin[g] .. row_begin[g+1]-1].  order: N, row_begin: num + 1 int32 on the device, apart
- * from each other and from row_adapter.  One bunch's grouping
- * serves every layer, forward and backward.  N <= 2^26, num <= 2^21, N * (num + 1) <= 2^40: it reads that many ids twice
- * (a bunch is what it is made for; 2^20 rows of 2000 adapters are 16 GB out of the caches). */
+ * order[row_begin[g] .. row_begin[g+1]-1].  order: N, row_begin: num + 1 int32 on the device, apart from
+ * each other and from row_adapter (else refused).  One bunch's grouping serves every layer, forward and backward.
+ * N <= 2^26, num <= 2^21, N * (num + 1) <= 2^40: it reads that many ids twice (it is made for bunches; 2^20 rows of
+ * 2000 adapters are 16 GB out of the caches). */
 int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int32_t num, int32_t *order,
                         int32_t *row_begin);
 
@@ -495,9 +495,9 @@ int hipI32_adapter_plan(khStream_t s, const int32_t *row_adapter, int32_t N, int
  *   out(N x O)       out[r,:] = act( bias + in[r,:] * W^T + t[r,:] * up_g )
  * with g = row_adapter[r].  `order` (may be NULL: the rows as they stand) is the sequence in which rows are put
  * together into tiles: give hipI32_adapter_plan's where neighbouring rows have different adapters, NULL where they lie
- * together already (utterances, single frames).  The result does not depend on it beyond rounding (t and out of a row
- * that a broken order does not list are undefined).  `t` is what the backward pass needs; bias may be NULL.  out and t must
- * not overlap each other or an input (refused; matrices side by side in the rows of a larger one do not overlap).
+ * together already (utterances, single frames).  The result does not depend on it beyond rounding (t and out of a
+ * row that a broken order does not list are undefined).  `t` is what the backward pass needs; bias may be NULL.  out
+ * and t must not overlap each other or an input (refused; matrices side by side in the rows of a larger one do not).
  * Rows behind N and columns behind O (max_rank) are left as they are; with O = 0 nothing is written.  N <= 2^26,
  * I <= 2^30, O <= 2^29.
  * Uses no library workspace: may be captured into a graph.  A row of t has the same bits whoever shares its call, and
@@ -523,7 +523,8 @@ int hipF_adapter_forward(khStream_t s, int act, int32_t N, int32_t O, int32_t I,
  * gradients to be whole (an entry outside is skipped).  An adapter without rows gets a gradient of zeros; rows of the
  * stacks outside every adapter are left as they are.  Sums are taken in a fixed order: the same call gives the same
  * bits.  Outputs must not overlap each other or an input that the call reads (refused).  N <= 2^26, O <= 2^30,
- * I <= 2^30 (2^29 with eout), num * max(I, O) / 32 < 2^23 with gradients.  The shared W is not updated here (hipF_affine_update). */
+ * I <= 2^30 (2^29 with eout), num * max(I, O) / 32 < 2^23 with gradients.  The shared W is not updated here
+ * (hipF_affine_update). */
 int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t I, const float *e, int32_t lde, const float *in,
                           int32_t ldin, const float *W, int32_t ldw, const khAdapters *ad, const int32_t *row_adapter,
                           const int32_t *order, const int32_t *row_begin, const float *t, int32_t ldt, float *u,
@@ -540,8 +541,8 @@ int hipF_adapter_backward(khStream_t s, int32_t N, int32_t O, int32_t I, const f
  * idx -1, val -inf.  lse[r] = log(sum_c exp(mat[r,c])) (may be NULL; -inf for a row of -inf, NaN for
  * one that holds a NaN or +inf), so that val - lse are log-posteriors.  What hipF_find_row_max_id is for one
  * maximum; it makes a teacher's outputs small enough to keep.  The outputs must not overlap each other or mat
- * (refused).  At most 2^30
- * columns.  Uses no library workspace. */
+ * (refused).  At most 2^30 columns.  Uses no library workspace.  Rows of nearly one value, nearly all masked or with a
+ * NaN or +inf take 3 to 40 times as long as others. */
 int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t K, int32_t *idx, int32_t ldidx, float *val,
                  int32_t ldval, float *lse);
 
@@ -551,14 +552,13 @@ int hipF_row_top(khStream_t s, const float *mat, MatrixDim d, int32_t K, int32_t
  *   p = softmax(x / T), p1 = softmax(x)
  *   row_loss = w * [ (1-h) * T^2 * sum_k q_k (log q_k - log p[idx_k])  +  h * (-log p1[label]) ]
  *   diff     = w * [ (1-h) * T * (p * (1 if there is an entry else 0) - q)  +  h * (p1 - onehot(label)) ]
- * diff is the derivative of row_loss with respect to x; it may be NULL (the loss alone) or be x
- * itself (same stride); else no output may overlap another or an input (refused).  A column named by two
- * entries gets both; an entry of -inf has q = 0 and 0 * log 0 = 0 (a row of nothing else has no
- * entry).  label (may be NULL when h is 0): a label outside
- * [0, cols) is none, its part of the row is zero.  w = weight[r] (NULL = 1); a row of weight 0, and a row whose x are
+ * diff is the derivative of row_loss with respect to x; it may be NULL (the loss alone) or be x itself
+ * (same stride); else no output may overlap another or an input (refused).  A column named by two entries gets both;
+ * an entry of -inf has q = 0 and 0 * log 0 = 0 (a row of nothing else has no entry).  label (may be NULL when h is 0):
+ * a label outside [0, cols) is none, its part of the row is zero.  w = weight[r] (NULL = 1); a row of weight 0, and a row whose x are
  * all -inf, get loss 0 and a gradient of zeros whatever the row holds.  row_loss (rows floats) may be NULL if loss is;
- * loss[0] += sum of row_loss (double on the device, summed in a fixed order: the same call gives the
- * same bits; may be NULL).  2^-126 <= T (no subnormal float), 0 <= h <= 1.
+ * loss[0] += sum of row_loss (double on the device, summed in a fixed order: the same call gives the same bits; may be
+ * NULL).  2^-126 <= T (no subnormal float), 0 <= h <= 1.
  * Sums in float over at most 1024 partial sums per row, the logarithms in double.  At most 2^30 columns.  Uses no library
  * workspace. */
 int hipF_distill_eval(khStream_t s, const float *x, MatrixDim d, const int32_t *idx, int32_t ldidx, const float *val,
